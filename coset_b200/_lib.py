@@ -78,6 +78,12 @@ SIGNATURES = {
     "coset_e8_layer_fake_quant_fwd": [_vp, _vp, _vp, _vp, _i64, _i64, _i32, _f32, _vp, _i32, _vp, _vp, _vp],
     "coset_e8_layer_fake_quant_bwd": [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _f32, _vp, _vp, _vp],
     "coset_e8_fake_quant_bwd": [_vp, _i32, _vp, _vp, _vp, _i64, _i64, _i32, _f32, _vp, _vp, _vp],
+    "coset_e8_cache_row_words": [_i32],
+    "coset_e8_cache_write": [_vp, _i64, _i32, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp],
+    "coset_e8_cache_read": [_vp, _i64, _i32, _i32, _i32, _vp, _i64, _vp, _vp, _i32, _vp],
+    "coset_e8_cache_attention_scratch_bytes": [_i32],
+    "coset_e8_cache_attention": [_vp, _i32, _i64, _i64, _i32, _i32, _vp, _i64, _i32, _i32, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _f32, _vp, _vp,
+                                 _vp, _i64, _vp],
 }
 
 

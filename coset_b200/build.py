@@ -35,6 +35,8 @@ SOURCES = [
     "e8_decode_gemm.cu",
     "e8_dense_gemm.cu",
     "f32_product.cu",
+    "e8_cache.cu",
+    "e8_cache_attention.cu",
     "d4.cu",
 ]
 

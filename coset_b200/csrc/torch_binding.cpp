@@ -21,6 +21,9 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <map>
+#include <mutex>
+
 #include "../../include/coset_b200.h"
 
 namespace {
@@ -750,11 +753,185 @@ PyObject* own_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- key/value cache
+struct CachePages {
+    const Tensor& t;
+    int64_t n_pages;
+    int n_heads, page_size, dim;
+};
+// [n_pages, n_heads, page_size, words]; the words of a row give its head_dim
+CachePages pages_arg(PyObject* o) {
+    const Tensor& t = cuda_arg(o, "pages");
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, "pages must be int32, got ", t.scalar_type());
+    TORCH_CHECK_VALUE(t.dim() == 4 && t.is_contiguous(), "pages must be a contiguous tensor [n_pages, n_heads, page_size, words]");
+    int dim = 0;
+    for (int d : {64, 128, 256})
+        if (t.size(3) == coset_e8_cache_row_words(d)) dim = d;
+    TORCH_CHECK_VALUE(dim != 0, "pages has rows of ", t.size(3), " words, which are those of no head_dim (64, 128 or 256)");
+    TORCH_CHECK_VALUE(t.size(1) >= 1 && t.size(1) <= 65535 && t.size(2) <= 1024 && t.size(0) <= INT32_MAX, "pages has sizes out of range: ", t.sizes());
+    return {t, t.size(0), (int)t.size(1), (int)t.size(2), dim};
+}
+void same_device(const Tensor& t, const Tensor& as, const char* name) {
+    TORCH_CHECK_VALUE(t.device() == as.device(), name, " is on ", t.device(), ", the pages are on ", as.device());
+}
+void no_gradient(const Tensor& t, const char* name) {
+    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name, " requires a gradient, and the cache has no backward pass: call under torch.no_grad()");
+}
+// A tensor of whole numbers of `type` with `dim` dimensions, its last one contiguous.
+const Tensor& index_arg(PyObject* o, const char* name, at::ScalarType type, int64_t dim, const Tensor& pages) {
+    const Tensor& t = cuda_arg(o, name);
+    TORCH_CHECK_TYPE(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
+    TORCH_CHECK_VALUE(t.dim() == dim, name, " must have ", dim, " dimension(s), got ", t.sizes());
+    same_device(t, pages, name);
+    return t;
+}
+// x [n, heads, dim] as rows that begin at multiples of 16 bytes
+Tensor cache_rows(const Tensor& x) {
+    const int64_t whole = 16 / x.element_size();
+    const bool fits = x.numel() == 0 || (x.stride(2) == 1 && x.stride(0) % whole == 0 && x.stride(1) % whole == 0 && (uintptr_t)x.data_ptr() % 16 == 0);
+    if (fits) return x;
+    return x.is_contiguous() ? x.clone() : x.contiguous();
+}
+
+// cache_write(pages, k, v, slots)
+PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    nargs_are(n, 4);
+    const CachePages p = pages_arg(a[0]);
+    const Tensor &k = cuda_arg(a[1], "k"), &v = cuda_arg(a[2], "v"), &slots = index_arg(a[3], "slots", at::kLong, 1, p.t);
+    TORCH_CHECK_VALUE(k.dim() == 3 && k.size(1) == p.n_heads && k.size(2) == p.dim, "k must be [n, ", p.n_heads, ", ", p.dim, "], got ", k.sizes());
+    TORCH_CHECK_VALUE(v.sizes() == k.sizes(), "v must have k's shape ", k.sizes(), ", got ", v.sizes());
+    TORCH_CHECK_VALUE(slots.size(0) == k.size(0), "expected ", k.size(0), " slots, got ", slots.size(0));
+    TORCH_CHECK_TYPE(v.scalar_type() == k.scalar_type(), "k and v must have the same type, got ", k.scalar_type(), " and ", v.scalar_type());
+    const int code = dtype_code(k, "k");
+    same_device(k, p.t, "k");
+    same_device(v, p.t, "v");
+    no_gradient(k, "k");
+    no_gradient(v, "v");
+    {
+        NoGil no_gil;
+        c10::cuda::CUDAGuard guard(p.t.device());
+        const Tensor kr = cache_rows(k), vr = cache_rows(v), at = contiguous(slots);
+        check_rc(coset_e8_cache_write(data(p.t), p.n_pages, p.n_heads, p.page_size, p.dim, data(kr), kr.stride(0), kr.stride(1), data(vr), vr.stride(0),
+                                      vr.stride(1), code, (const int64_t*)data(at), k.size(0), stream_of(p.t)), "coset_e8_cache_write");
+    }
+    written(p.t);
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* pair_of(const Tensor& x, const Tensor& y) {
+    PyObject* pair = PyTuple_New(2);
+    if (!pair) throw python_error();
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(x));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(y));
+    return pair;
+}
+
+// cache_read(pages, slots, dtype_code) -> (k, v)
+PyObject* cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    nargs_are(n, 3);
+    const CachePages p = pages_arg(a[0]);
+    const Tensor& slots = index_arg(a[1], "slots", at::kLong, 1, p.t);
+    const int code = (int)int_arg(a[2]);
+    const at::ScalarType type = scalar_type(code);
+    Tensor k, v;
+    {
+        NoGil no_gil;
+        c10::cuda::CUDAGuard guard(p.t.device());
+        const Tensor at = contiguous(slots);
+        k = empty({at.size(0), p.n_heads, p.dim}, type, p.t);
+        v = empty({at.size(0), p.n_heads, p.dim}, type, p.t);
+        check_rc(coset_e8_cache_read(data(p.t), p.n_pages, p.n_heads, p.page_size, p.dim, (const int64_t*)data(at), at.size(0), data(k), data(v), code,
+                                     stream_of(p.t)), "coset_e8_cache_read");
+    }
+    return pair_of(k, v);
+    END_HANDLE_TH_ERRORS
+}
+
+// The attention's scratch: kept for each stream, whose calls follow one another.  A capture gets one of its own, cleared in the graph, so that a
+// replay shares it with no other call.
+Tensor attention_scratch(int64_t bytes, const Tensor& like) {
+    const auto fresh = [&]() { return empty({bytes}, at::kByte, like).zero_(); };
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(like.get_device()).stream();
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return fresh();
+    static std::mutex mutex;
+    static auto* kept = new std::map<std::pair<int, cudaStream_t>, Tensor>();  // never destroyed: the driver may be gone before static objects are
+    const std::lock_guard<std::mutex> lock(mutex);
+    Tensor& t = (*kept)[{(int)like.get_device(), stream}];
+    if (!t.defined() || t.numel() < bytes) {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        const c10::InferenceMode normal(false);
+        t = fresh();
+    }
+    return t;
+}
+
+// cache_attention(q, pages, table, lens, q_starts or None, tree or None, scale, return_lse, out or None) -> out or (out, lse)
+PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    nargs_are(n, 9);
+    const CachePages p = pages_arg(a[1]);
+    const Tensor &q = cuda_arg(a[0], "q"), &table = index_arg(a[2], "table", at::kInt, 2, p.t), &lens = index_arg(a[3], "lens", at::kInt, 1, p.t);
+    TORCH_CHECK_VALUE(q.dim() == 3 && q.size(2) == p.dim && q.size(1) >= 1 && q.size(1) % p.n_heads == 0, "q must be [n, heads, ", p.dim,
+                      "] with heads a multiple of the cache's ", p.n_heads, ", got ", q.sizes());
+    const int64_t seqs = lens.size(0), queries = q.size(0);
+    TORCH_CHECK_VALUE(table.size(0) == seqs, "table has ", table.size(0), " rows for ", seqs, " sequences");
+    TORCH_CHECK_VALUE(table.size(1) <= INT32_MAX && seqs < INT32_MAX && queries <= INT32_MAX && q.size(1) <= INT32_MAX, "a size is out of range");
+    const int code = dtype_code(q, "q");
+    same_device(q, p.t, "q");
+    no_gradient(q, "q");
+    Tensor starts, tree;
+    if (a[4] != Py_None) {
+        starts = index_arg(a[4], "q_starts", at::kInt, 1, p.t);
+        TORCH_CHECK_VALUE(starts.size(0) == seqs + 1, "q_starts must have ", seqs + 1, " values, got ", starts.size(0));
+    } else {
+        TORCH_CHECK_VALUE(seqs > 0 ? queries % seqs == 0 : queries == 0, queries, " queries are not shared evenly by ", seqs, " sequences: q_starts says whose they are");
+    }
+    if (a[5] != Py_None) {
+        tree = index_arg(a[5], "tree", at::kLong, 1, p.t);
+        TORCH_CHECK_VALUE(tree.size(0) == queries, "tree must have ", queries, " words, got ", tree.size(0));
+        TORCH_CHECK_VALUE(starts.defined() || seqs == 0 || queries / seqs <= 64, "a tree has at most 64 queried tokens per sequence, got ", queries / (seqs ? seqs : 1));
+    }
+    const float scale = (float)float_arg(a[6]);
+    const bool want_lse = a[7] == Py_True;
+    Tensor out = optional_arg(a[8], "out"), lse;
+    if (out.defined()) {
+        TORCH_CHECK_TYPE(out.scalar_type() == q.scalar_type(), "out must have q's type ", q.scalar_type(), ", got ", out.scalar_type());
+        TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.is_contiguous() && out.device() == q.device(), "out has the wrong shape, layout or device");
+        TORCH_CHECK_VALUE((uintptr_t)out.data_ptr() % 16 == 0, "out must be 16-byte aligned");
+        TORCH_CHECK_VALUE(!out.is_alias_of(q), "out shares its memory with q");
+        no_gradient(out, "out");
+    }
+    const bool given = out.defined();
+    {
+        NoGil no_gil;
+        c10::cuda::CUDAGuard guard(p.t.device());
+        const Tensor qr = cache_rows(q), pages_of = table.stride(1) == 1 || table.size(1) <= 1 ? table : table.contiguous(), len = contiguous(lens);
+        if (starts.defined()) starts = contiguous(starts);
+        if (tree.defined()) tree = contiguous(tree);
+        if (!given) out = empty(q.sizes(), q.scalar_type(), q);
+        if (want_lse) lse = empty({queries, q.size(1)}, at::kFloat, q);
+        const int64_t bytes = coset_e8_cache_attention_scratch_bytes(p.dim);
+        const Tensor scratch = queries > 0 ? attention_scratch(bytes, q) : Tensor();
+        check_rc(coset_e8_cache_attention(data(qr), code, qr.stride(0), qr.stride(1), (int)queries, (int)q.size(1), data(p.t), p.n_pages, p.n_heads, p.page_size,
+                                          p.dim, (const int32_t*)data(pages_of), pages_of.stride(0), (int)pages_of.size(1), (const int32_t*)data(len),
+                                          starts.defined() ? (const int32_t*)data(starts) : nullptr, (int)seqs, tree.defined() ? (const int64_t*)data(tree) : nullptr,
+                                          scale, data(out), want_lse ? fdata(lse) : nullptr, scratch.defined() ? scratch.data_ptr() : nullptr, bytes,
+                                          stream_of(p.t)), "coset_e8_cache_attention");
+    }
+    if (given) written(out);
+    return want_lse ? pair_of(out, lse) : THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 #define COSET_METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     COSET_METHOD(encode_packed), COSET_METHOD(decode_packed), COSET_METHOD(encode_digits), COSET_METHOD(decode_digits), COSET_METHOD(quantize),
     COSET_METHOD(grad_encode), COSET_METHOD(decode_mean), COSET_METHOD(vlut_linear), COSET_METHOD(vlut_layout), COSET_METHOD(vlut_product), COSET_METHOD(vlut_product_checked),
-    COSET_METHOD(decode_gemm), COSET_METHOD(dense_linear), COSET_METHOD(layer_fake_quant), COSET_METHOD(qat_linear), COSET_METHOD(own_product), COSET_METHOD(own_product_sizes), {nullptr, nullptr, 0, nullptr}};
+    COSET_METHOD(decode_gemm), COSET_METHOD(dense_linear), COSET_METHOD(layer_fake_quant), COSET_METHOD(qat_linear), COSET_METHOD(own_product), COSET_METHOD(own_product_sizes),
+    COSET_METHOD(cache_write), COSET_METHOD(cache_read), COSET_METHOD(cache_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_coset_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -435,6 +435,48 @@ int coset_f32_linear(const float* x, const float* w, const float* bias, int T, i
 int coset_f32_input_grad(const float* g, const float* w, int T, int n_out, int n_in, float* dx, void* stream);
 int coset_f32_weight_grad(const float* g, const float* x, int T, int n_out, int n_in, float* dw, void* stream);
 
+/*
+ * E8-coded key/value cache.  (No counterpart in the reference.)  A row is the head_dim (64, 128 or 256) values of one token and one head.
+ * Its step is the smallest bf16 number >= max|x| / 7; its values, in steps and rounded to 1/4096, are replaced by the nearest point of E8
+ * block by block: f + c / 2 with f in [-8, 7] per value and one bit c per block of 8.  Where several are as near, the whole-number point stands, and
+ * in a block whose sum is odd the first of the coordinates that are as far moves.  A row below 2^-100 is stored as zeros; one
+ * that holds an infinity or a NaN reads back as NaN.
+ *   pages  : [n_pages, n_heads] records of page_size * coset_e8_cache_row_words(head_dim) 32-bit words, 16-byte aligned; page_size is a power
+ *            of two from 16 to 1024.  A record is page_size rows of key codes (head_dim / 8 words each, f + 8 of value i of a block in bits
+ *            4i..4i+3), of value codes, of key heads (ceil(head_dim / 128) words: the step in the high half, the c of 16 blocks in the low
+ *            half, block b at bit b % 16; both words of a row of 256 hold the step), and of value heads.
+ *   slots  : [n_tokens] place of each token, page * page_size + offset.  Negative, or behind the last page: nothing is written, and zeros
+ *            are read.  The slots of one write differ from each other.
+ *   k, v   : write: rows at k + token * k_token_stride + head * k_head_stride (elements), 16-byte aligned; read: [n_tokens, n_heads, head_dim]
+ * dtype is that of k and v; a value that is read is rounded once from the exact product (f + c / 2) * step.
+ */
+int coset_e8_cache_row_words(int head_dim);
+int coset_e8_cache_write(void* pages, int64_t n_pages, int n_heads, int page_size, int head_dim, const void* k, int64_t k_token_stride,
+                         int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, int dtype, const int64_t* slots,
+                         int64_t n_tokens, void* stream);
+int coset_e8_cache_read(const void* pages, int64_t n_pages, int n_heads, int page_size, int head_dim, const int64_t* slots, int64_t n_tokens,
+                        void* k, void* v, int dtype, void* stream);
+
+/*
+ * Attention of the last tokens of every sequence (one generated token, a chain or a tree of drafted ones) over an E8-coded cache that holds
+ * them already: out = softmax(scale * q K^T + mask) V, lse = log(sum(exp(scale * q K^T + mask))).
+ *   q      : [n_queries, q_heads, head_dim] float32 or bf16 (rows 16-byte aligned, strides in elements); head h reads cache head
+ *            h / (q_heads / n_heads)
+ *   table  : [n_seqs, table_stride] pages of each sequence, max_pages of them counted; tokens on a page outside [0, n_pages) are not seen
+ *   lens   : [n_seqs] tokens of each sequence in the cache, the queried ones last (cut to max_pages * page_size)
+ *   q_starts: [n_seqs + 1] first query of each sequence, ascending; null: n_queries / n_seqs each.  Rows of no sequence are left as they were.
+ *   tree   : [n_queries] bit j: the query sees queried token j of its sequence (itself among them; tokens from 64 on are not seen).  null: a chain,
+ *            every query sees the queried tokens up to itself.  All earlier tokens of the sequence are seen by all its queries.
+ *   out    : [n_queries, q_heads, head_dim] of q's type;  lse: [n_queries, q_heads] float32, may be null
+ * A query that sees nothing gives zeros and -infinity.  scratch: coset_e8_cache_attention_scratch_bytes(head_dim) bytes, 16-byte aligned, zero
+ * before the first use and left so by every call; calls that may overlap on the device need one each.  One launch; sums are float32.
+ */
+int64_t coset_e8_cache_attention_scratch_bytes(int head_dim);
+int coset_e8_cache_attention(const void* q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int n_queries, int q_heads, const void* pages,
+                             int64_t n_pages, int n_heads, int page_size, int head_dim, const int32_t* table, int64_t table_stride, int max_pages,
+                             const int32_t* lens, const int32_t* q_starts, int n_seqs, const int64_t* tree, float scale, void* out, float* lse,
+                             void* scratch, int64_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
