@@ -2,11 +2,11 @@
 // sequence, which are one generated token, a chain or a tree of drafted ones.  Few rows: some queries per cache head.
 //
 // Nothing dense is made.  A key is step (f + c / 2) with f + 8 a 4-bit number n, so
-//     q k / step = sum_i q_i n_i + sum_blocks c_b (sum of q over b) / 2 - 8 sum_i q_i.
-// A nibble in a byte of its own IS the 8-bit floating-point number (e4m3) n 2^-9, so an operand of the 8-bit products costs three instructions per
-// word of eight; they run at twice the rate of the 16-bit ones and their sums are float32.  A bf16 query is the sum of two e4m3 numbers: exactly, down to 2^-9
-// of its row's largest value, and to 2^-17 of that below.  A float32 query is three, and three more for what these leave, 2^12 times as large
-// and summed apart.  The bits c go through the 16-bit products, as powers of two made by placing a bit in the exponent's field.
+//     q k / step = sum_i q_i n_i + sum_blocks c_b (sum of q over b) / 2 - 8 sum_i q_i,
+// and with q in fixed point (16 bits below the largest of a bf16 row, 24 of a float32 one, a power of two per row) all of it is a sum of products of
+// bytes: three instructions make eight operands of a word of codes, the sums are exact in 32 bits, and start from the bits of 1.5 2^23, so that they are read
+// as floating-point numbers.  What a bf16 query loses is 2^-16 of its row's largest value, and nothing down to 2^-8 of it.  (As 8-bit floating-point
+// numbers, which a nibble is too, the products are no instruction of this chip but fourteen.)
 //     sum_j w_j v_j, w_j = p_j step_j, takes 16-bit products: a nibble under the exponent of 1024 (or 64, four bits up) less 1032 (72) is f.  (As the
 // subnormal number that its bits are it would need no subtraction, but the tensor cores line up products by their exponents and drop ten bits of such a
 // sum: results 1e-3 off.  Without the subtraction the sums' rounding, towards zero, counts 72 times: sum w f is small against sum w.)
@@ -23,8 +23,6 @@
 //
 // The running maximum is that of a weight times the size of its value (s + the exponent of the value's step), so that w = p step fits 16 bits: what is
 // lost is below 2^-31 of the row's largest.  It follows only when it lags by 2^kSlack.  For float32 queries w is split into two 16-bit numbers.
-#include <cuda_fp8.h>
-
 #include "e8_cache_attention.cuh"
 
 using namespace coset;
@@ -35,7 +33,9 @@ namespace {
 constexpr int kUnit = 32;         // tokens of a warp's step
 constexpr int kLeastUnits = 4;    // of a CTA
 constexpr int kLeastSize = -90;   // exponent of a value's step as far as the running maximum goes: sums of p / 2^kLeastSize stay finite
-constexpr int kMostCtas = 192;    // counters in the scratch memory
+constexpr int kMostCtas = 152;    // counters in the scratch memory
+constexpr int kExact = 0x4B400000;  // the bits of kExactly = 1.5 2^23; a whole number of up to 22 bits added to them is added to it
+constexpr float kExactly = 12582912.0f;
 
 // The row of a group of 8 that stands in row r of an operand: 0 1 2 3 5 4 7 6.  With the swizzles below no read of codes has a bank conflict.
 __device__ __forceinline__ int placed(int r) { return r ^ ((r >> 2) & 1); }
@@ -46,7 +46,7 @@ struct Shape {
     static constexpr int kKeyWords = DIM / 32;    // words of a row that a lane has for S
     static constexpr int kValueWords = DIM / 64;  // for O
     static constexpr int kTiles = DIM / 16;       // of O^T
-    static constexpr int kBitTiles = DIM == 256 ? 2 : 1;
+    static constexpr int kBitTiles = DIM == 256 ? 2 : 1;  // of the blocks' bits, for S and for O
     static constexpr int kStage = 2 * kUnit * (kRowBytes + 4 * kHeads);
     // where 16-byte chunk c of row r lies
     static __device__ __forceinline__ int chunk(int r, int c) { return DIM == 64 ? c : DIM == 128 ? c ^ (r & 2) : c ^ (r & 7); }
@@ -56,9 +56,15 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// bytes without a sign by bytes with one (the top part of a query) or without
+template <bool SIGNED>
+__device__ __forceinline__ void mma_bytes(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (SIGNED)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // f = n - 8 of the nibbles at bits 0..3 (even) or 4..7 (odd) of both halves of x, as 16-bit numbers
 __device__ __forceinline__ uint32_t even_values(uint32_t x) {
@@ -95,66 +101,57 @@ __device__ __forceinline__ uint32_t rest_pair(float lo, float hi, uint32_t pair)
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
     return half_pair(lo - f.x, hi - f.y);
 }
-// The e4m3 numbers nearest to x, y, z, w in a word; they become what is left.
-__device__ __forceinline__ uint32_t take_bytes(float (&x)[4]) {
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-        const __nv_fp8x2_storage_t b = __nv_cvt_float2_to_fp8x2(make_float2(x[i], x[i + 1]), __NV_SATFINITE, __NV_E4M3);
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(b, __NV_E4M3);
-        const float2 f = __half22float2(__half2(h));
-        x[i] -= f.x;
-        x[i + 1] -= f.y;
-        word |= (uint32_t)b << (8 * i);
-    }
-    return word;
-}
 // Where bit b of four stands in the exponent of a 16-bit number, and the number that it is there: bit 10 + b, 2^-14, 2^-13, 2^-11, 2^-7.
 __device__ __forceinline__ float of_bit(int b) { return b == 0 ? 0x1p-14f : b == 1 ? 0x1p-13f : b == 2 ? 0x1p-11f : 0x1p-7f; }
+// Bits 0..3 of x as the bytes of a word
+__device__ __forceinline__ uint32_t bytes_of_bits(uint32_t x) { return (x & 15u) * 0x00204081u & 0x01010101u; }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
 
 template <int WORDS>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[WORDS]);
-template <>
-__device__ __forceinline__ void load_words<1>(const uint8_t* p, uint32_t (&w)[1]) { w[0] = *reinterpret_cast<const uint32_t*>(p); }
-template <>
-__device__ __forceinline__ void load_words<2>(const uint8_t* p, uint32_t (&w)[2]) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x; w[1] = v.y;
-}
-template <>
-__device__ __forceinline__ void load_words<4>(const uint8_t* p, uint32_t (&w)[4]) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
+    if (WORDS == 1) {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if (WORDS == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x; w[1] = v.y;
+    } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    }
 }
 
-// A tile of queries of one head in shared memory, in the order of the operands.
+// A tile of queries of one head in shared memory, in the order of the operands.  Part 0 of a number is its top byte, with the sign.
 template <int DIM, int PARTS, int NB>
 struct Queries {
-    static constexpr int kPairs = PARTS == 2 ? 3 : 1;  // of e4m3 numbers for a query
-    uint4 words[NB][kPairs][DIM / 32][32];  // of the operand's word w: values 0, 2, 4, 6 and 1, 3, 5, 7, first the one part, then the other
-    uint32_t blocks[NB][DIM / 32][32];      // the sum over block w in two 16-bit parts
-    float start[8 * NB];                    // -8 sum of q
-    float factor[8 * NB];                   // from a sum to a score in powers of two, but for the key's step
-    uint64_t bits[8 * NB];                  // the queried tokens that a query sees
+    uint2 words[NB][PARTS][DIM / 32][32];                 // of word w: values 0, 2, 4, 6 and 1, 3, 5, 7 of its block
+    uint2 blocks[NB][PARTS][Shape<DIM>::kBitTiles][32];   // half the sums of four blocks: the part's bytes, and 64ths of what the top part is too small for
+    int start[PARTS][8 * NB];                             // kExact - 8 sum of the part
+    float factor[8 * NB];                                 // from a sum to a score in powers of two, but for the key's step
+    uint64_t bits[8 * NB];                                // the queried tokens that a query sees
 };
 
 template <int DIM, int NB, int WARPS>
 struct Joining {
     static constexpr int kStride = DIM * 18 / 16 + 4;  // rows of 16 values lie 18 apart: no bank conflicts between lanes
     float o[WARPS][8][kStride];
-    float m[WARPS][8 * NB], l[WARPS][8 * NB];
+    float m[8 * NB][WARPS], l[8 * NB][WARPS];  // of the warps; then m is the factor that brings a warp's sums to the row's maximum
+    float top[8 * NB], sum[8 * NB];
     static __device__ __forceinline__ int at(int d) { return d + 2 * (d / 16); }
+};
+// The same memory when the CTAs' parts are joined
+template <int NB>
+struct JoiningCtas {
+    float m[kMostCtas][8 * NB], l[kMostCtas][8 * NB];
 };
 
 template <int DIM, int PARTS, int NB, int WARPS>
 struct Layout {
     static constexpr int kStages = 2;
-    static constexpr int kRing = 0;
-    static constexpr int kQueries = kRing + WARPS * kStages * Shape<DIM>::kStage;
+    static constexpr int kQueries = WARPS * kStages * Shape<DIM>::kStage;
     static constexpr int kJoining = kQueries + (int)sizeof(Queries<DIM, PARTS, NB>);
     static constexpr int kBytes = kJoining + (int)sizeof(Joining<DIM, NB, WARPS>);
+    static_assert(sizeof(JoiningCtas<NB>) <= sizeof(Joining<DIM, NB, WARPS>::o), "shared memory");
 };
 
 // A place in the CTA's row of units: tile `tile` of `tiles` of (seq, head, query tile).
@@ -165,7 +162,7 @@ struct Place {
 template <int ROWS>
 __device__ __forceinline__ void enter(const Attend& a, Place& p) {
     p.s = sequence(a, p.seq);
-    p.qtiles = (int)(((int64_t)p.s.count * a.group + ROWS - 1) / ROWS);
+    p.qtiles = (p.s.count * a.group + ROWS - 1) / ROWS;
     p.tiles = max((p.s.len + kUnit - 1) / kUnit, 1);
 }
 template <int ROWS>
@@ -185,20 +182,14 @@ __device__ __forceinline__ void next_segment(const Attend& a, Place& p) {
 template <int ROWS, int WARPS>
 struct Cursor {
     Place place;
-    int64_t left = 0;  // units of the CTA from the segment's first one here on
+    int left = 0;      // units of the CTA from the segment's first one here on
     int i = 0, n = 0;  // unit in the segment's part that the CTA has, and their number
     int page[2] = {-1, -1};
-    __device__ __forceinline__ void look_up(const Attend& a) {
-        if (left <= 0) return;
-        const int token = (place.tile + i) * kUnit;
-        page[0] = page_of(a, place.seq, token, place.s.len);
-        page[1] = page_of(a, place.seq, token + 16, place.s.len);
-    }
-    __device__ __forceinline__ void begin(const Attend& a, const Place& p, int64_t units, int warp) {
+    __device__ __forceinline__ void begin(const Attend& a, const Place& p, int units, int warp) {
         place = p;
         left = units;
         i = warp;
-        n = (int)min((int64_t)(place.tiles - place.tile), left);
+        n = min(place.tiles - place.tile, left);
         settle(a, warp);
     }
     __device__ __forceinline__ void settle(const Attend& a, int warp) {
@@ -207,14 +198,26 @@ struct Cursor {
             if (left <= 0) return;
             next_segment<ROWS>(a, place);
             i = warp;
-            n = (int)min((int64_t)place.tiles, left);
+            n = min(place.tiles, left);
         }
-        look_up(a);
+        const int token = (place.tile + i) * kUnit;
+        page[0] = page_of(a, place.seq, token, place.s.len);
+        page[1] = page_of(a, place.seq, token + 16, place.s.len);
+    }
+};
+
+// The units' cut: CTA c has base units, and one more where c < more.
+struct Cut {
+    int base, more;
+    __device__ __forceinline__ int from(int cta) const { return base * cta + min(cta, more); }
+    __device__ __forceinline__ int cta_of(int unit) const {
+        const int longer = more * (base + 1);
+        return unit < longer ? unit / (base + 1) : more + (unit - longer) / base;
     }
 };
 
 template <int DIM, int PARTS, int NB, int WARPS>
-__device__ __forceinline__ void load_queries(const Attend& a, const Place& p, Queries<DIM, PARTS, NB>& s, int q_bf16) {
+__device__ __forceinline__ void load_queries(const Attend& a, const Place& p, Queries<DIM, PARTS, NB>& s) {
     constexpr int kBlocks = DIM / 8;
     const int rows = min(8 * NB, p.s.count * a.group - p.qtile * 8 * NB);
     for (int at = threadIdx.x; at < 8 * NB * kBlocks; at += 32 * WARPS) {  // whole warps go round together
@@ -223,9 +226,10 @@ __device__ __forceinline__ void load_queries(const Attend& a, const Place& p, Qu
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+        uint64_t bits = 0;
         if (r < rows) {
             const int64_t e = (p.s.first + query) * a.q_token_stride + q_head * a.q_head_stride + 8 * b;
-            if (q_bf16) {
+            if (PARTS == 2) {
                 const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + e));
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -234,69 +238,69 @@ __device__ __forceinline__ void load_queries(const Attend& a, const Place& p, Qu
                 const float4 v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + e)), w = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + e) + 1);
                 x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
             }
+            if (b == 0) bits = a.tree ? (uint64_t)__ldg(a.tree + p.s.first + query) : (uint64_t)query;
         }
         uint32_t most = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);
 #pragma unroll
         for (int m = 1; m < kBlocks; m *= 2) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, m));
-        // a power of two that brings the row's largest into [2^7, 2^8): e4m3 ends at 448, and the sum over a block, 16 times as large, fits 16 bits
+        // fixed point: a power of two brings the row's largest into [2^(8 PARTS - 2), 2^(8 PARTS - 1))
+        constexpr int kTop = 8 * PARTS - 1;
         const bool number = most < 0x7F800000u;
-        const int exponent = number ? min(7 - ((int)(most >> 23) - 127), 126) : 0;
+        const int exponent = number ? min(kTop - 1 - ((int)(most >> 23) - 127), 126) : 0;
         const float up = __uint_as_float((uint32_t)(exponent + 127) << 23);
-        float sum = 0.0f;
+        int q[8], total[PARTS], sum = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            x[i] = number ? x[i] * up : 0.0f;
-            sum += x[i];
+            q[i] = number ? min(__float2int_rn(x[i] * up), (1 << kTop) - 1) : 0;
+            sum += q[i];
         }
-        const int t = b / (DIM / 32), word = b % (DIM / 32), lane = (r % 8) * 4 + t;
-        float even[4] = {x[0], x[2], x[4], x[6]}, odd[4] = {x[1], x[3], x[5], x[7]};
-        uint32_t part[2 * Queries<DIM, PARTS, NB>::kPairs][2];
+        const int lane = (r % 8) * 4 + b / (DIM / 32), word = b % (DIM / 32);
 #pragma unroll
-        for (int i = 0; i < 2 * Queries<DIM, PARTS, NB>::kPairs; ++i) {
-            if (i == 3) {
+        for (int j = 0; j < PARTS; ++j) {
+            const int shift = 8 * (PARTS - 1 - j);
+            uint32_t even = 0, odd = 0;
+            total[j] = 0;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) { even[k] *= 4096.0f; odd[k] *= 4096.0f; }
+            for (int i = 0; i < 8; ++i) {
+                const int part = j == 0 ? q[i] >> shift : q[i] >> shift & 255;
+                total[j] += part;
+                (i & 1 ? odd : even) |= (uint32_t)(part & 255) << (4 * (i & 6));
             }
-            part[i][0] = take_bytes(even);
-            part[i][1] = take_bytes(odd);
+            s.words[r / 8][j][word][lane] = make_uint2(even, odd);
+#pragma unroll
+            for (int m = 1; m < kBlocks; m *= 2) total[j] += __shfl_xor_sync(0xFFFFFFFFu, total[j], m);
+            // four neighbours have the bytes of a word of the blocks' sums; with 64 values there are two, and the others are zero
+            const int half = (sum + 1) >> 1, part = j == 0 ? half >> shift : half >> shift & 255;
+            uint32_t low = j == 0 ? part & 63 : part, high = j == 0 ? part >> 6 & 255 : 0;
+            low <<= 8 * (word & 3);
+            high <<= 8 * (word & 3);
+#pragma unroll
+            for (int m = 1; m < (DIM == 64 ? 2 : 4); m *= 2) {
+                low |= __shfl_xor_sync(0xFFFFFFFFu, low, m);
+                high |= __shfl_xor_sync(0xFFFFFFFFu, high, m);
+            }
+            if ((word & 3) == 0) s.blocks[r / 8][j][word / 4][lane] = make_uint2(low, high);
+            if (b == 0) s.start[j][r] = kExact - 8 * total[j];
         }
-#pragma unroll
-        for (int i = 0; i < Queries<DIM, PARTS, NB>::kPairs; ++i)
-            s.words[r / 8][i][word][lane] = make_uint4(part[2 * i][0], part[2 * i][1], part[2 * i + 1][0], part[2 * i + 1][1]);
-        float total = 0.0f;  // of what the parts stand for, so that what they leave is not counted eight times
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float unit = PARTS == 2 ? 0x1p-12f : 1.0f;
-            total += (x[2 * i] - even[i] * unit) + (x[2 * i + 1] - odd[i] * unit);
-        }
-#pragma unroll
-        for (int m = 1; m < kBlocks; m *= 2) total += __shfl_xor_sync(0xFFFFFFFFu, total, m);
-        const float half = sum * (0x1p-10f / of_bit(word & 3));
-        const uint32_t first = half_pair(half, 0.0f);
-        s.blocks[r / 8][word][lane] = (first & 0xFFFFu) | (rest_pair(half, 0.0f, first) << 16);
         if (b == 0) {
-            s.start[r] = -8.0f * 0x1p-9f * total;
-            s.factor[r] = number ? 0x1p9f * (a.scale * 1.44269504f) / up : __uint_as_float(0x7FC00000u);
-            uint64_t bits = 0;
-            if (r < rows) bits = a.tree ? (uint64_t)__ldg(a.tree + p.s.first + query) : 0;
-            s.bits[r] = a.tree ? bits : (uint64_t)query;
+            s.factor[r] = number ? a.scale * 1.44269504f / up : __uint_as_float(0x7FC00000u);
+            s.bits[r] = bits;
         }
     }
 }
 
 template <int DIM, int PARTS, int NB, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, 1)
-k_cache_attend(const __grid_constant__ Attend a, int q_bf16) {
+k_cache_attend(const __grid_constant__ Attend a) {
     using S = Shape<DIM>;
     using L = Layout<DIM, PARTS, NB, WARPS>;
-    constexpr int kRows = 8 * NB, kThreads = 32 * WARPS;
-    constexpr float kSlack = PARTS == 2 ? 2.0f : 8.0f, kShift = PARTS == 2 ? 12.0f : 6.0f;  // weights reach 2^(1 + kSlack + kShift)
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int64_t scan[WARPS + 1];
-    __shared__ int64_t found_before;
-    __shared__ int found_seq, is_last;
+    constexpr int kRows = 8 * NB, kThreads = 32 * WARPS, kWeights = PARTS - 1;  // 16-bit parts of a weight
+    constexpr float kSlack = PARTS == 3 ? 2.0f : 8.0f, kShift = PARTS == 3 ? 12.0f : 6.0f;  // weights reach 2^(1 + kSlack + kShift)
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int64_t scan[WARPS];
+    __shared__ int found_seq, found_before, is_last;
     auto& queries = *reinterpret_cast<Queries<DIM, PARTS, NB>*>(smem + L::kQueries);
     auto& joining = *reinterpret_cast<Joining<DIM, NB, WARPS>*>(smem + L::kJoining);
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -304,7 +308,6 @@ k_cache_attend(const __grid_constant__ Attend a, int q_bf16) {
     grid_trigger();
 
     // ---- this CTA's units
-    int64_t total = 0, before = 0;
     const auto units_of = [&](int b) {
         if (b >= a.n_seqs) return (int64_t)0;
         Place p;
@@ -312,7 +315,7 @@ k_cache_attend(const __grid_constant__ Attend a, int q_bf16) {
         enter<kRows>(a, p);
         return (int64_t)p.qtiles * a.pages.n_heads * p.tiles;
     };
-    // inclusive sum over the threads; *sum: over all of them
+    // sum over this and the threads before; *sum: over all of them
     const auto inclusive = [&](int64_t v, int64_t* sum) {
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -331,77 +334,78 @@ k_cache_attend(const __grid_constant__ Attend a, int q_bf16) {
         *sum = all;
         return v + mine;
     };
-    int64_t units = units_of(threadIdx.x), upto = inclusive(units, &total);
+    if (threadIdx.x == 0) found_seq = -1;
+    int64_t all, units = units_of(threadIdx.x), upto = inclusive(units, &all);
+    const int64_t first_sum = all;
     for (int b = kThreads; b < a.n_seqs; b += kThreads) {
         int64_t more;
         inclusive(units_of(b + threadIdx.x), &more);
-        total += more;
+        all += more;
     }
-    const int64_t ctas = min((int64_t)gridDim.x, (total + kLeastUnits - 1) / kLeastUnits);
+    if (all < 1 || all > INT32_MAX) return;  // so many only from starts that overlap: the host refuses as much work
+    const int total = (int)all, ctas = min((int)gridDim.x, (total - 1) / kLeastUnits + 1);
     if (blockIdx.x >= ctas) return;
-    const int64_t from = total * blockIdx.x / ctas, to = total * (blockIdx.x + 1) / ctas;
-    if (threadIdx.x == 0) found_seq = -1;
-    for (int b = 0; b < a.n_seqs; b += kThreads) {
+    const Cut cut = {total / ctas, total % ctas};
+    const int from = cut.from(blockIdx.x), to = cut.from(blockIdx.x + 1);
+    int64_t before = 0, sum = first_sum;
+    for (int b = 0;; before += sum) {
         if (b > 0) {
-            int64_t sum;
             units = units_of(b + threadIdx.x);
             upto = inclusive(units, &sum) + before;
-            if (threadIdx.x == 0) scan[WARPS] = before + sum;
-        } else if (threadIdx.x == kThreads - 1) {
-            scan[WARPS] = upto;
         }
-        __syncthreads();
-        before = scan[WARPS];
         if (upto - units <= from && from < upto) {
             found_seq = b + threadIdx.x;
-            found_before = upto - units;
+            found_before = (int)(upto - units);
         }
         __syncthreads();
-        if (found_seq >= 0) break;
+        b += kThreads;
+        if (found_seq >= 0 || b >= a.n_seqs) break;
     }
     Place place;
     place.seq = found_seq;
     enter<kRows>(a, place);
     {
-        const int64_t segment = (from - found_before) / place.tiles;
-        place.tile = (int)((from - found_before) % place.tiles);
-        place.head = (int)(segment / place.qtiles);
-        place.qtile = (int)(segment % place.qtiles);
+        const int segment = (from - found_before) / place.tiles;
+        place.tile = (from - found_before) % place.tiles;
+        place.head = segment / place.qtiles;
+        place.qtile = segment % place.qtiles;
     }
 
     // ---- fetching
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + L::kRing + warp * L::kStages * S::kStage;
-    const uint8_t* ring_at = smem + L::kRing + warp * L::kStages * S::kStage;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * L::kStages * S::kStage;
+    const uint8_t* ring_at = smem + warp * L::kStages * S::kStage;
     Cursor<kRows, WARPS> cursor;
-    const int page_mask = (1 << a.pages.page_log2) - 1;
+    const int page_log2 = a.pages.page_log2, page_mask = (1 << page_log2) - 1;
+    const uint32_t record_chunks = (row_words(DIM) * 4 / 8) << (page_log2 - 1);  // 16-byte chunks; rows are multiples of 8 bytes, pages of 16 rows
+    const uint32_t to_chunk = ring + (lane / S::kChunks) * S::kRowBytes + 16 * S::chunk(lane / S::kChunks, lane % S::kChunks);
+    const uint32_t to_odd_chunk = ring + (lane / S::kChunks) * S::kRowBytes + 16 * S::chunk(lane / S::kChunks + 4, lane % S::kChunks);
+    const uint32_t to_head = ring + 2 * kUnit * S::kRowBytes + ((lane / 16) * kUnit + lane % 16) * S::kHeads * 4;
+    const uint32_t from_head = (2 * S::kRowBytes + (lane / 16) * S::kHeads * 4 << page_log2) + lane % 16 * S::kHeads * 4;
     // Fetches the next unit; bit h of the result: its tokens 16 h .. 16 h + 15 have a page.
     const auto fetch = [&](int stage) {
         int there = 0;
         if (cursor.left > 0) {
-            const uint32_t dst = ring + stage * S::kStage;
             const int token = (cursor.place.tile + cursor.i) * kUnit;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int page = cursor.page[h];
                 if (page < 0) continue;
                 there |= 1 << h;
-                const uint32_t* rec = a.pages.words + record<DIM>(a.pages, page, cursor.place.head);
-                const int row0 = (token + 16 * h) & page_mask;
+                const uint64_t chunk = ((uint64_t)(uint32_t)page * (uint32_t)a.pages.n_heads + (uint32_t)cursor.place.head) * record_chunks;
+                const uint8_t* rec = reinterpret_cast<const uint8_t*>(a.pages.words) + chunk * 16;
+                const uint32_t row0 = (uint32_t)(token + 16 * h) & page_mask;
+                const uint8_t* key = rec + row0 * S::kRowBytes + lane * 16;
+                const uint8_t* value = key + ((uint32_t)S::kRowBytes << page_log2);
+                const uint8_t* head = rec + row0 * S::kHeads * 4 + from_head;
+                const uint32_t dst = stage * S::kStage + 16 * h * S::kRowBytes;
 #pragma unroll
-                for (int which = 0; which < 2; ++which) {
-                    const uint8_t* src = reinterpret_cast<const uint8_t*>(rec) + ((int64_t)which << a.pages.page_log2) * S::kRowBytes + row0 * S::kRowBytes;
-#pragma unroll
-                    for (int i = 0; i < 16 * S::kChunks; i += 32) {
-                        const int at = i + lane, r = at / S::kChunks, c = at % S::kChunks;
-                        copy16(dst + (which * kUnit + 16 * h + r) * S::kRowBytes + 16 * S::chunk(r, c), src + at * 16);
-                    }
+                for (int i = 0; i < S::kRowBytes / 32; ++i) {  // 32 chunks, 32 / kChunks rows at a time
+                    const uint32_t at = (DIM == 256 && (i & 1) ? to_odd_chunk : to_chunk) + dst + i * 512;  // four rows of 256 further the swizzle differs
+                    copy16(at, key + i * 512);
+                    copy16(at + kUnit * S::kRowBytes, value + i * 512);
                 }
-                // heads: of the keys by the first half of the lanes, of the values by the second
-                const int which = lane / 16, r = lane % 16;
-                const uint32_t* src = rec + ((2 * code_words(DIM) + which * S::kHeads) << a.pages.page_log2) + (row0 + r) * S::kHeads;
 #pragma unroll
-                for (int i = 0; i < S::kHeads; ++i)
-                    copy4(dst + 2 * kUnit * S::kRowBytes + ((which * kUnit + 16 * h + r) * S::kHeads + i) * 4, src + i);
+                for (int i = 0; i < S::kHeads; ++i) copy4(to_head + stage * S::kStage + (16 * h * S::kHeads + i) * 4, head + 4 * i);
             }
             cursor.i += WARPS;
             cursor.settle(a, warp);
@@ -413,10 +417,10 @@ k_cache_attend(const __grid_constant__ Attend a, int q_bf16) {
     int stage = 0, there = fetch(0);
 
     // ---- one (sequence, head, tile of queries) after the other
-    for (int64_t unit = from; unit < to;) {
-        const int n = (int)min((int64_t)(place.tiles - place.tile), to - unit);
+    for (int unit = from; unit < to;) {
+        const int n = min(place.tiles - place.tile, to - unit);
         __syncthreads();  // nobody reads the queries before, nor joins any more
-        load_queries<DIM, PARTS, NB, WARPS>(a, place, queries, q_bf16);
+        load_queries<DIM, PARTS, NB, WARPS>(a, place, queries);
         __syncthreads();
         float o[NB][S::kTiles][4], bits[NB][S::kBitTiles][4], m[NB][2], l[NB][2];
 #pragma unroll
@@ -443,161 +447,158 @@ k_cache_attend(const __grid_constant__ Attend a, int q_bf16) {
             const int token0 = (place.tile + i) * kUnit;
 
             // scores: [group of 16 tokens][tile of 8 queries][token g: query 2 t, 2 t + 1; token g + 8: the same]
-            float s[2][NB][4], rest[2][NB][4];  // rest: 2^12 times what the first three parts of a float32 query leave
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                const float s0 = queries.start[8 * nb + 2 * t], s1 = queries.start[8 * nb + 2 * t + 1];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    s[h][nb][0] = s[h][nb][2] = s0;
-                    s[h][nb][1] = s[h][nb][3] = s1;
-                    rest[h][nb][0] = rest[h][nb][1] = rest[h][nb][2] = rest[h][nb][3] = 0.0f;
-                }
-            }
-            uint32_t kw[2][2][S::kKeyWords], kh[2][2];
+            float s[2][NB][4], step[2][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                int sum[PARTS][NB][4];
+#pragma unroll
+                for (int j = 0; j < PARTS; ++j)
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const int2 s0 = *reinterpret_cast<const int2*>(&queries.start[j][8 * nb + 2 * t]);
+                        sum[j][nb][0] = sum[j][nb][2] = s0.x;
+                        sum[j][nb][1] = sum[j][nb][3] = s0.y;
+                    }
+                uint32_t kw[2][S::kKeyWords], kh[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int r = 16 * h + 8 * e + placed(g);
                     const uint8_t* row = at + r * S::kRowBytes;
                     if (DIM == 64) {
-                        load_words<S::kKeyWords < 4 ? S::kKeyWords : 1>(row + 8 * t, reinterpret_cast<uint32_t(&)[S::kKeyWords < 4 ? S::kKeyWords : 1]>(kw[h][e]));
+                        load_words<2>(row + 8 * t, kw[e]);
                     } else {
 #pragma unroll
-                        for (int c = 0; c < S::kKeyWords / 4; ++c)
-                            load_words<4>(row + 16 * S::chunk(r, t * (S::kKeyWords / 4) + c), reinterpret_cast<uint32_t(&)[4]>(kw[h][e][c * 4]));
+                        for (int c = 0; c < S::kKeyWords / 4; ++c) load_words<4>(row + 16 * S::chunk(r, t * (S::kKeyWords / 4) + c), kw[e] + c * 4);
                     }
-                    kh[h][e] = key_heads[r * S::kHeads + (DIM == 256 ? t / 2 : 0)];
+                    kh[e] = key_heads[r * S::kHeads + (DIM == 256 ? t / 2 : 0)];
+                    step[h][e] = __uint_as_float(kh[e] & 0xFFFF0000u);
                 }
-            }
 #pragma unroll
-            for (int w = 0; w < S::kKeyWords; ++w) {
-                uint32_t x[2][4];
+                for (int w = 0; w < S::kKeyWords; ++w) {
+                    const uint32_t x0 = kw[0][w] & 0x0F0F0F0Fu, x1 = kw[1][w] & 0x0F0F0F0Fu, x2 = kw[0][w] >> 4 & 0x0F0F0F0Fu, x3 = kw[1][w] >> 4 & 0x0F0F0F0Fu;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    x[h][0] = kw[h][0][w] & 0x0F0F0F0Fu;
-                    x[h][1] = kw[h][1][w] & 0x0F0F0F0Fu;
-                    x[h][2] = kw[h][0][w] >> 4 & 0x0F0F0F0Fu;
-                    x[h][3] = kw[h][1][w] >> 4 & 0x0F0F0F0Fu;
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int j = 0; j < PARTS; ++j) {
+                            const uint2 q = queries.words[nb][j][w][lane];
+                            if (j == 0) mma_bytes<true>(sum[j][nb], x0, x1, x2, x3, q.x, q.y);
+                            else mma_bytes<false>(sum[j][nb], x0, x1, x2, x3, q.x, q.y);
+                        }
+                }
+#pragma unroll
+                for (int k = 0; k < S::kBitTiles; ++k) {
+                    const int shift = (DIM == 64 ? 2 * t : DIM == 128 ? 4 * t : 8 * (t & 1)) + 4 * k;
+                    const uint32_t x0 = bytes_of_bits(kh[0] >> shift), x1 = bytes_of_bits(kh[1] >> shift);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int j = 0; j < PARTS; ++j) {
+                            const uint2 q = queries.blocks[nb][j][k][lane];
+                            if (j == 0) mma_bytes<true>(sum[j][nb], x0, x1, x0 * 64, x1 * 64, q.x, q.y);
+                            else mma_bytes<false>(sum[j][nb], x0, x1, x0, x1, q.x, 0);
+                        }
                 }
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int pair = 0; pair < (PARTS == 2 ? 3 : 1); ++pair) {
-                        const uint4 q = queries.words[nb][pair][w][lane];
+                    for (int i4 = 0; i4 < 4; ++i4) {
+                        float x = __int_as_float(sum[0][nb][i4]) - kExactly;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            mma8(2 * pair < 3 ? s[h][nb] : rest[h][nb], x[h][0], x[h][1], x[h][2], x[h][3], q.x, q.y);
-                            mma8(2 * pair + 1 < 3 ? s[h][nb] : rest[h][nb], x[h][0], x[h][1], x[h][2], x[h][3], q.z, q.w);
-                        }
+                        for (int j = 1; j < PARTS; ++j) x = __fmaf_rn(x, 256.0f, __int_as_float(sum[j][nb][i4]) - kExactly);
+                        s[h][nb][i4] = x * step[h][i4 / 2];
                     }
-            }
-#pragma unroll
-            for (int w = 0; w < S::kKeyWords; w += 2) {
-                uint32_t x[2][2];  // the lane's bits of this and the next blocks at bit 10 and following of both halves
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        x[h][e] = __byte_perm(kh[h][e], 0, 0x1010) >> ((DIM == 64 ? 2 * t : DIM == 128 ? 4 * t : 8 * (t & 1)) + (w & ~3)) << 10;
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const uint32_t q0 = queries.blocks[nb][w][lane], q1 = queries.blocks[nb][w + 1][lane];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        mma(s[h][nb], x[h][0] & (0x04000400u << (w & 3)), x[h][1] & (0x04000400u << (w & 3)), x[h][0] & (0x08000800u << (w & 3)),
-                            x[h][1] & (0x08000800u << (w & 3)), q0, q1);
-                }
             }
 
             // softmax
-            const bool all = token0 + kUnit <= drafted && there == 3;
-            float step[2][2], value_step[2][2], size[2][2];
+            uint32_t p[2][NB][2][kWeights];  // weights as 16-bit pairs of queries, [group][tile][token g, g + 8][part]
+            const auto softmax = [&](auto every) {
+                constexpr bool kAll = decltype(every)::value;
+                uint32_t seen[NB];  // bit 4 h + 2 e + c: token 16 h + 8 e + g is seen by query 2 t + c
+                if (!kAll) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                    for (int nb = 0; nb < NB; ++nb) {
+                        seen[nb] = 0;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    step[h][e] = __uint_as_float(kh[h][e] & 0xFFFF0000u);
-                    const uint32_t v = value_heads[(16 * h + 8 * e + placed(g)) * S::kHeads];
-                    value_step[h][e] = __uint_as_float(v & 0xFFFF0000u);
-                    size[h][e] = (float)max((int)(v >> 23 & 255u) - 127, kLeastSize);
-                }
-            uint32_t seen[NB] = {};  // bit 4 h + 2 e + c: token 16 h + 8 e + g is seen by query 2 t + c
-            if (!all) {
+                        for (int c = 0; c < 2; ++c) {
+                            const uint64_t who = queries.bits[8 * nb + 2 * t + c];
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
+                            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const uint64_t who = queries.bits[8 * nb + 2 * t + c];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int token = token0 + 16 * h + 8 * e + placed(g), j = token - drafted;
-                                const bool yes = token < place.s.len && (there >> h & 1) &&
-                                                 (j < 0 || (a.tree ? j < 64 && (who >> j & 1) : j <= (int)who));
-                                seen[nb] |= (uint32_t)yes << (4 * h + 2 * e + c);
-                            }
-                    }
-            }
-            uint32_t p[2][NB][2][PARTS];  // weights as 16-bit pairs of queries, [group][tile][token g, g + 8][part]
-            float lag = -INFINITY, top[NB][2];
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const float f = queries.factor[8 * nb + 2 * t + c];
-                    top[nb][c] = -INFINITY;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float& x = s[h][nb][2 * e + c];
-                            if (PARTS == 2) x += rest[h][nb][2 * e + c] * 0x1p-12f;
-                            x *= step[h][e];
-                            if (all || (seen[nb] >> (4 * h + 2 * e + c) & 1)) top[nb][c] = larger(top[nb][c], __fmaf_rn(x, f, size[h][e]));
+                                for (int e = 0; e < 2; ++e) {
+                                    const int token = token0 + 16 * h + 8 * e + placed(g), j = token - drafted;
+                                    const bool yes = token < place.s.len && (there >> h & 1) &&
+                                                     (j < 0 || (a.tree ? j < 64 && (who >> j & 1) : j <= (int)who));
+                                    seen[nb] |= (uint32_t)yes << (4 * h + 2 * e + c);
+                                }
                         }
-                    if (top[nb][c] != -INFINITY) lag = larger(lag, top[nb][c] - kShift - m[nb][c]);
-                }
-            if (__any_sync(0xFFFFFFFFu, !(lag <= kSlack))) {
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float x = top[nb][c];
-#pragma unroll
-                        for (int d = 4; d < 32; d *= 2) x = larger(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
-                        x = larger(m[nb][c], x - kShift);
-                        const float keep = x == -INFINITY ? 1.0f : exp2_of(m[nb][c] - x);
-                        m[nb][c] = x;
-                        l[nb][c] *= keep;
-#pragma unroll
-                        for (int k = 0; k < S::kTiles; ++k) { o[nb][k][c] *= keep; o[nb][k][c + 2] *= keep; }
-#pragma unroll
-                        for (int k = 0; k < S::kBitTiles; ++k) { bits[nb][k][c] *= keep; bits[nb][k][c + 2] *= keep; }
                     }
-            }
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                const float f[2] = {queries.factor[8 * nb + 2 * t], queries.factor[8 * nb + 2 * t + 1]};
+                }
+                const auto sees = [&](int nb, int h, int e, int c) { return kAll || (seen[nb] >> (4 * h + 2 * e + c) & 1); };
+                float value_step[2][2], size[2][2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float w[2];
+                        const uint32_t v = value_heads[(16 * h + 8 * e + placed(g)) * S::kHeads];
+                        value_step[h][e] = __uint_as_float(v & 0xFFFF0000u);
+                        size[h][e] = fmaxf(__uint_as_float(0x4B400000u + (v >> 23 & 255u)) - (kExactly + 127.0f), (float)kLeastSize);
+                    }
+                float lag = -INFINITY, top[NB][2], f[NB][2];
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const float2 factor = *reinterpret_cast<const float2*>(&queries.factor[8 * nb + 2 * t]);
+                    f[nb][0] = factor.x;
+                    f[nb][1] = factor.y;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        top[nb][c] = -INFINITY;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                if (sees(nb, h, e, c)) top[nb][c] = larger(top[nb][c], __fmaf_rn(s[h][nb][2 * e + c], f[nb][c], size[h][e]));
+                        if (kAll || top[nb][c] != -INFINITY) lag = larger(lag, top[nb][c] - m[nb][c]);
+                    }
+                }
+                if (__any_sync(0xFFFFFFFFu, !(lag <= kSlack + kShift))) {
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float x = exp2_of(__fmaf_rn(s[h][nb][2 * e + c], f[c], -m[nb][c]));
-                            w[c] = x * value_step[h][e];
-                            if (!all && !(seen[nb] >> (4 * h + 2 * e + c) & 1)) x = w[c] = 0.0f;
-                            l[nb][c] += x;
+                            float x = top[nb][c];
+#pragma unroll
+                            for (int d = 4; d < 32; d *= 2) x = larger(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
+                            x = larger(m[nb][c], x - kShift);
+                            const float keep = x == -INFINITY ? 1.0f : exp2_of(m[nb][c] - x);
+                            m[nb][c] = x;
+                            l[nb][c] *= keep;
+#pragma unroll
+                            for (int k = 0; k < S::kTiles; ++k) { o[nb][k][c] *= keep; o[nb][k][c + 2] *= keep; }
+#pragma unroll
+                            for (int k = 0; k < S::kBitTiles; ++k) { bits[nb][k][c] *= keep; bits[nb][k][c + 2] *= keep; }
                         }
-                        const uint32_t pair = half_pair(w[0], w[1]);
-                        p[h][nb][e][0] = transposed(pair);
-                        if (PARTS == 2) p[h][nb][e][PARTS - 1] = transposed(rest_pair(w[0], w[1], pair));
-                    }
-            }
+                }
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float w[2];
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                float x = exp2_of(__fmaf_rn(s[h][nb][2 * e + c], f[nb][c], -m[nb][c]));
+                                w[c] = x * value_step[h][e];
+                                if (!sees(nb, h, e, c)) x = w[c] = 0.0f;
+                                l[nb][c] += x;
+                            }
+                            const uint32_t pair = half_pair(w[0], w[1]);
+                            p[h][nb][e][0] = transposed(pair);
+                            if (kWeights == 2) p[h][nb][e][kWeights - 1] = transposed(rest_pair(w[0], w[1], pair));
+                        }
+            };
+            if (token0 + kUnit <= drafted && there == 3) softmax(std::true_type());
+            else softmax(std::false_type());
 
             // values
 #pragma unroll
@@ -615,7 +616,7 @@ k_cache_attend(const __grid_constant__ Attend a, int q_bf16) {
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                        for (int part = 0; part < PARTS; ++part) mma(acc[nb][tile], a0, a1, a2, a3, p[h][nb][0][part], p[h][nb][1][part]);
+                        for (int part = 0; part < kWeights; ++part) mma(acc[nb][tile], a0, a1, a2, a3, p[h][nb][0][part], p[h][nb][1][part]);
                 };
 #pragma unroll
                 for (int w = 0; w < S::kValueWords; ++w)
@@ -630,7 +631,7 @@ k_cache_attend(const __grid_constant__ Attend a, int q_bf16) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int part = 0; part < PARTS; ++part)
+                    for (int part = 0; part < kWeights; ++part)
 #pragma unroll
                         for (int k = 0; k < S::kBitTiles; ++k)
                             mma(bits[nb][k], x & (0x04000400u << (2 * k)), x & (0x08000800u << (2 * k)), y & (0x04000400u << (2 * k)), y & (0x08000800u << (2 * k)),
@@ -640,10 +641,9 @@ k_cache_attend(const __grid_constant__ Attend a, int q_bf16) {
             there = there_next;
         }
 
-        // ---- the warps' parts into one, tile of 8 queries by tile
-        const int64_t first_unit = unit - place.tile, end_unit = first_unit + place.tiles;  // of the segment, whoever has them
+        // ---- the warps' parts into one
         const bool whole = place.tile == 0 && n == place.tiles;
-        const int rows = min(kRows, place.s.count * a.group - place.qtile * kRows);
+        const int rows = min(kRows, place.s.count * a.group - place.qtile * kRows), live = min(n, WARPS);  // the first `live` warps had units
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -652,90 +652,131 @@ k_cache_attend(const __grid_constant__ Attend a, int q_bf16) {
 #pragma unroll
                 for (int d = 4; d < 32; d *= 2) x += __shfl_xor_sync(0xFFFFFFFFu, x, d);
                 if (g == 0) {
-                    joining.m[warp][8 * nb + 2 * t + c] = m[nb][c];
-                    joining.l[warp][8 * nb + 2 * t + c] = x;
+                    joining.m[8 * nb + 2 * t + c][warp] = m[nb][c];
+                    joining.l[8 * nb + 2 * t + c][warp] = x;
                 }
             }
         __syncthreads();
-        const int slot = place.tile > 0 ? 0 : 1;  // a segment that began before this CTA, or one that goes on behind it
-        float* partial = a.partials + ((int64_t)blockIdx.x * 2 + slot) * kRows * (DIM + 2);
+        if (threadIdx.x < kRows) {
+            float top = -INFINITY, sum = 0.0f;
+            for (int w = 0; w < live; ++w) top = larger(top, joining.m[threadIdx.x][w]);
+            for (int w = 0; w < live; ++w) {
+                const float its = joining.m[threadIdx.x][w], keep = its == -INFINITY ? 0.0f : exp2_of(its - top);
+                joining.m[threadIdx.x][w] = keep;
+                if (keep != 0.0f) sum += joining.l[threadIdx.x][w] * keep;
+            }
+            joining.top[threadIdx.x] = top;
+            joining.sum[threadIdx.x] = sum;
+        }
+        __syncthreads();
         const int q_heads = a.group * a.pages.n_heads;
         // row r of the tile: where its result goes
         const auto row_of = [&](int r) {
             const int row = place.qtile * kRows + r;
             return (int64_t)(place.s.first + row / a.group) * q_heads + place.head * a.group + row % a.group;
         };
-        const auto put = [&](int r, int d, float v) {
-            if (q_bf16) static_cast<__nv_bfloat16*>(a.out)[row_of(r) * DIM + d] = __float2bfloat16_rn(v);
-            else static_cast<float*>(a.out)[row_of(r) * DIM + d] = v;
+        const auto put = [&](int r, int d, float x, float y) {
+            if (PARTS == 2) *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + row_of(r) * DIM + d) = __floats2bfloat162_rn(x, y);
+            else *reinterpret_cast<float2*>(static_cast<float*>(a.out) + row_of(r) * DIM + d) = make_float2(x, y);
         };
+        const auto put_lse = [&](int r, float top, float sum) {
+            if (a.lse) a.lse[row_of(r)] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * 0.69314718f;
+        };
+        // a CTA's parts: of the segment that began before it, and of the one that goes on behind it
+        constexpr int kPart = kRows * (DIM + 2);
+        float* partial = a.partials + ((int64_t)blockIdx.x * 2 + (place.tile > 0 ? 0 : 1)) * kPart;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            float scale[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float x = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) x = larger(x, joining.m[w][8 * nb + 2 * t + c]);
-                scale[c] = m[nb][c] == -INFINITY ? 0.0f : exp2_of(m[nb][c] - x);
-            }
             if (nb > 0) __syncthreads();  // the tile before is read
+            if (warp < live) {
+                float scale[2];
 #pragma unroll
-            for (int k = 0; k < S::kTiles; ++k) {
-                const int d = g * (DIM / 8) + 2 * k, block = k / 4;  // of the lane's blocks
+                for (int c = 0; c < 2; ++c) scale[c] = joining.m[8 * nb + 2 * t + c][warp];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const float half = bits[nb][block / 2][c + 2 * (block & 1)] * (0.5f / of_bit(block));
-                    float2 v = make_float2((o[nb][k][c] + half) * scale[c], (o[nb][k][c + 2] + half) * scale[c]);
-                    if (scale[c] == 0.0f) v = make_float2(0.0f, 0.0f);
-                    *reinterpret_cast<float2*>(&joining.o[warp][2 * t + c][joining.at(d)]) = v;
+                for (int k = 0; k < S::kTiles; ++k) {
+                    const int d = g * (DIM / 8) + 2 * k, block = k / 4;  // of the lane's blocks
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float half = bits[nb][block / 2][c + 2 * (block & 1)] * (0.5f / of_bit(block));
+                        float2 v = make_float2((o[nb][k][c] + half) * scale[c], (o[nb][k][c + 2] + half) * scale[c]);
+                        if (scale[c] == 0.0f) v = make_float2(0.0f, 0.0f);
+                        *reinterpret_cast<float2*>(&joining.o[warp][2 * t + c][joining.at(d)]) = v;
+                    }
                 }
             }
             __syncthreads();
-            for (int at = threadIdx.x; at < 8 * DIM; at += kThreads) {
-                const int r = 8 * nb + at / DIM, d = at % DIM;
+            for (int at = threadIdx.x; at < 8 * DIM / 2; at += kThreads) {
+                const int r = 8 * nb + at / (DIM / 2), d = at % (DIM / 2) * 2;
                 if (r >= rows) continue;
-                float v = 0.0f, top = -INFINITY, sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    v += joining.o[w][at / DIM][joining.at(d)];
-                    top = larger(top, joining.m[w][r]);
+                float2 v = make_float2(0.0f, 0.0f);
+                for (int w = 0; w < live; ++w) {
+                    const float2 x = *reinterpret_cast<const float2*>(&joining.o[w][r % 8][joining.at(d)]);
+                    v.x += x.x;
+                    v.y += x.y;
                 }
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) sum += joining.m[w][r] == -INFINITY ? 0.0f : joining.l[w][r] * exp2_of(joining.m[w][r] - top);
+                const float top = joining.top[r], sum = joining.sum[r];
                 if (whole) {
-                    put(r, d, top == -INFINITY ? 0.0f : v / sum);
-                    if (d == 0 && a.lse) a.lse[row_of(r)] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * 0.69314718f;
+                    put(r, d, top == -INFINITY ? 0.0f : v.x / sum, top == -INFINITY ? 0.0f : v.y / sum);
+                    if (d == 0) put_lse(r, top, sum);
                 } else {
-                    partial[r * (DIM + 2) + d] = v;
-                    if (d == 0) { partial[r * (DIM + 2) + DIM] = top; partial[r * (DIM + 2) + DIM + 1] = sum; }
+                    *reinterpret_cast<float2*>(partial + 2 * kRows + r * DIM + d) = v;
+                    if (d == 0) {
+                        partial[r] = top;
+                        partial[kRows + r] = sum;
+                    }
                 }
             }
         }
+        // ---- the CTAs' parts into one: those from the CTA with the segment's first unit to the one with its last
         if (!whole) {
-            // the CTAs that share the segment: the one with its first unit to the one with its last
-            const int64_t first_cta = ((first_unit + 1) * ctas - 1) / total, last_cta = (end_unit * ctas - 1) / total;
+            const int first_cta = cut.cta_of(unit - place.tile), parts = cut.cta_of(unit - place.tile + place.tiles - 1) - first_cta + 1;
             __threadfence();
             __syncthreads();
-            if (threadIdx.x == 0) is_last = atomicAdd(a.counters + first_cta, 1u) == (uint32_t)(last_cta - first_cta);
+            if (threadIdx.x == 0) is_last = atomicAdd(a.counters + first_cta, 1u) == (uint32_t)(parts - 1);
             __syncthreads();
             if (is_last) {
                 __threadfence();
-                const auto part = [&](int64_t cta) { return a.partials + (cta * 2 + (cta == first_cta ? 1 : 0)) * kRows * (DIM + 2); };
-                for (int at = threadIdx.x; at < rows * DIM; at += kThreads) {
-                    const int r = at / DIM, d = at % DIM;
-                    float top = -INFINITY, v = 0.0f, sum = 0.0f;
-                    for (int64_t cta = first_cta; cta <= last_cta; ++cta) top = larger(top, __ldcg(part(cta) + r * (DIM + 2) + DIM));
-                    for (int64_t cta = first_cta; cta <= last_cta; ++cta) {
-                        const float* x = part(cta) + r * (DIM + 2);
-                        const float its = __ldcg(x + DIM), keep = its == -INFINITY ? 0.0f : exp2_of(its - top);
-                        if (its != -INFINITY) {
-                            v += __ldcg(x + d) * keep;
-                            sum += __ldcg(x + DIM + 1) * keep;
+                auto& ctas_parts = *reinterpret_cast<JoiningCtas<NB>*>(joining.o);
+                const auto part = [&](int i) { return a.partials + ((int64_t)(first_cta + i) * 2 + (i == 0 ? 1 : 0)) * kPart; };
+                for (int at = threadIdx.x; at < parts * kRows; at += kThreads) {
+                    const int i = at / kRows, r = at % kRows;
+                    ctas_parts.m[i][r] = __ldcg(part(i) + r);
+                    ctas_parts.l[i][r] = __ldcg(part(i) + kRows + r);
+                }
+                __syncthreads();
+                for (int r = warp; r < rows; r += WARPS) {
+                    float top = -INFINITY, sum = 0.0f;
+                    for (int i = lane; i < parts; i += 32) top = larger(top, ctas_parts.m[i][r]);
+#pragma unroll
+                    for (int d = 1; d < 32; d *= 2) top = larger(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                    for (int i = lane; i < parts; i += 32) {
+                        const float its = ctas_parts.m[i][r], keep = its == -INFINITY ? 0.0f : exp2_of(its - top);
+                        ctas_parts.m[i][r] = keep;
+                        if (keep != 0.0f) sum += ctas_parts.l[i][r] * keep;
+                    }
+#pragma unroll
+                    for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+                    if (lane == 0) {
+                        joining.top[r] = top;
+                        joining.sum[r] = sum;
+                    }
+                }
+                __syncthreads();
+                for (int at = threadIdx.x; at < rows * (DIM / 2); at += kThreads) {
+                    const int r = at / (DIM / 2), d = at % (DIM / 2) * 2;
+                    float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll 8
+                    for (int i = 0; i < parts; ++i) {
+                        const float2 x = __ldcg(reinterpret_cast<const float2*>(part(i) + 2 * kRows + r * DIM + d));
+                        const float keep = ctas_parts.m[i][r];
+                        if (keep != 0.0f) {
+                            v.x += x.x * keep;
+                            v.y += x.y * keep;
                         }
                     }
-                    put(r, d, top == -INFINITY ? 0.0f : v / sum);
-                    if (d == 0 && a.lse) a.lse[row_of(r)] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * 0.69314718f;
+                    const float top = joining.top[r], sum = joining.sum[r];
+                    put(r, d, top == -INFINITY ? 0.0f : v.x / sum, top == -INFINITY ? 0.0f : v.y / sum);
+                    if (d == 0) put_lse(r, top, sum);
                 }
                 if (threadIdx.x == 0) a.counters[first_cta] = 0;
             }
@@ -750,21 +791,21 @@ constexpr int kMostRows = 16;
 int64_t scratch_bytes_of(int head_dim) { return 4 * kMostCtas + (int64_t)kMostCtas * 2 * kMostRows * (head_dim + 2) * 4; }
 
 template <int DIM, int PARTS, int NB, int WARPS>
-int launch_as(const Attend& a, int q_bf16, cudaStream_t st) {
+int launch_as(const Attend& a, cudaStream_t st) {
     using L = Layout<DIM, PARTS, NB, WARPS>;
     static_assert(L::kBytes <= 227 * 1024 - 1024, "shared memory");
     static_assert(8 * NB <= kMostRows, "scratch memory");
     const auto kernel = k_cache_attend<DIM, PARTS, NB, WARPS>;
     if (int e = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes), "cudaFuncSetAttribute")) return e;
     const int sms = sm_count(), grid = sms < kMostCtas ? sms : kMostCtas;
-    return launch_dependent("e8_cache_attention", kernel, (unsigned)grid, 32 * WARPS, L::kBytes, st, a, q_bf16);
+    return launch_dependent("e8_cache_attention", kernel, (unsigned)grid, 32 * WARPS, L::kBytes, st, a);
 }
 
 template <int DIM, int PARTS>
-int launch(const Attend& a, int q_bf16, cudaStream_t st) {
+int launch(const Attend& a, cudaStream_t st) {
     const int64_t rows = ((int64_t)a.n_queries + a.n_seqs - 1) / a.n_seqs * a.group;  // of a cache head, on average
-    if (rows <= 8) return launch_as<DIM, PARTS, 1, DIM == 256 ? 8 : 16>(a, q_bf16, st);
-    return launch_as<DIM, PARTS, 2, DIM == 256 && PARTS == 2 ? 6 : 8>(a, q_bf16, st);
+    if (rows <= 8) return launch_as<DIM, PARTS, 1, DIM == 256 ? 8 : 16>(a, st);
+    return launch_as<DIM, PARTS, 2, DIM == 256 && PARTS == 3 ? 6 : 8>(a, st);
 }
 
 }  // namespace
@@ -789,6 +830,9 @@ int coset_e8_cache_attention(const void* q, int dtype, int64_t q_token_stride, i
     if ((int64_t)max_pages * page_size > INT32_MAX - 64) return fail(COSET_E_UNSUPPORTED, "a sequence of 2^31 or more tokens");
     if ((int64_t)n_queries * q_heads > INT32_MAX - 64) return fail(COSET_E_UNSUPPORTED, "too many rows for one call");
     if (n_seqs == 0) return 0;
+    // no more than this many units are cut among the CTAs, however the queries are shared among the sequences
+    const int64_t tiles = ((int64_t)n_queries * (q_heads / n_heads) + 7) / 8 + n_seqs, longest = ((int64_t)max_pages * page_size + kUnit - 1) / kUnit + 1;
+    if ((double)tiles * n_heads * longest > 2e9) return fail(COSET_E_UNSUPPORTED, "too much work for one call: queries x pages of the table");
     const int64_t whole = dtype == COSET_DTYPE_F32 ? 4 : 8;
     if (!aligned(q, 16) || !aligned(out, 16) || (q_token_stride | q_head_stride) % whole) return fail(COSET_E_ALIGN, "rows of q and out must be 16-byte aligned");
     if (!scratch || scratch_bytes < coset_e8_cache_attention_scratch_bytes(head_dim)) return fail(COSET_E_BADARG, "scratch is null or too small");
@@ -800,9 +844,9 @@ int coset_e8_cache_attention(const void* q, int dtype, int64_t q_token_stride, i
     a.partials = (float*)scratch + kMostCtas;
     cudaStream_t st = (cudaStream_t)stream;
     const int bf16 = dtype == COSET_DTYPE_BF16;
-    if (head_dim == 64) return bf16 ? launch<64, 1>(a, 1, st) : launch<64, 2>(a, 0, st);
-    if (head_dim == 128) return bf16 ? launch<128, 1>(a, 1, st) : launch<128, 2>(a, 0, st);
-    return bf16 ? launch<256, 1>(a, 1, st) : launch<256, 2>(a, 0, st);
+    if (head_dim == 64) return bf16 ? launch<64, 2>(a, st) : launch<64, 3>(a, st);
+    if (head_dim == 128) return bf16 ? launch<128, 2>(a, st) : launch<128, 3>(a, st);
+    return bf16 ? launch<256, 2>(a, st) : launch<256, 3>(a, st);
 }
 
 }  // extern "C"
