@@ -18,12 +18,14 @@
 //
 // Work is cut into units of 32 tokens of one (sequence, head, tile of queries), and the units of all of them in a row are cut evenly among the CTAs, one
 // per SM; the lengths are read on the device, so a captured launch follows them.  A warp runs through its units alone, with the running maximum
-// and sum of the softmax in registers and the next unit's words on their way (cp.async); the warps of a CTA are joined in shared memory, and where
-// several CTAs share a row the last one to arrive joins them in the order of the CTAs.
+// and sum of the softmax in registers; one more warp, a lane for each of the others, looks up pages and brings the next units' codes by TMA (128-byte
+// swizzle), so that the addresses cost the others nothing.  The warps of a CTA are joined in shared memory, and where several CTAs share a row the last one
+// to arrive joins them in the order of the CTAs.
 //
 // The running maximum is that of a weight times the size of its value (s + the exponent of the value's step), so that w = p step fits 16 bits: what is
 // lost is below 2^-31 of the row's largest.  It follows only when it lags by 2^kSlack.  For float32 queries w is split into two 16-bit numbers.
 #include "e8_cache_attention.cuh"
+#include "umma.cuh"
 
 using namespace coset;
 using namespace coset::cache;
@@ -37,19 +39,27 @@ constexpr int kMostCtas = 152;    // counters in the scratch memory
 constexpr int kExact = 0x4B400000;  // the bits of kExactly = 1.5 2^23; a whole number of up to 22 bits added to them is added to it
 constexpr float kExactly = 12582912.0f;
 
-// The row of a group of 8 that stands in row r of an operand: 0 1 2 3 5 4 7 6.  With the swizzles below no read of codes has a bank conflict.
-__device__ __forceinline__ int placed(int r) { return r ^ ((r >> 2) & 1); }
-
+// A unit in shared memory: keys, values (lines of 128 bytes as they are in a page, one or several rows each, swizzled), their heads apart.
 template <int DIM>
 struct Shape {
-    static constexpr int kRowBytes = DIM / 2, kChunks = kRowBytes / 16, kHeads = head_words(DIM);
+    static constexpr int kRowBytes = DIM / 2, kHeads = head_words(DIM);
     static constexpr int kKeyWords = DIM / 32;    // words of a row that a lane has for S
     static constexpr int kValueWords = DIM / 64;  // for O
     static constexpr int kTiles = DIM / 16;       // of O^T
     static constexpr int kBitTiles = DIM == 256 ? 2 : 1;  // of the blocks' bits, for S and for O
-    static constexpr int kStage = 2 * kUnit * (kRowBytes + 4 * kHeads);
-    // where 16-byte chunk c of row r lies
-    static __device__ __forceinline__ int chunk(int r, int c) { return DIM == 64 ? c : DIM == 128 ? c ^ (r & 2) : c ^ (r & 7); }
+    static constexpr int kLines = 16 * kRowBytes / 128;   // of 16 tokens
+    static constexpr int kPlane = DIM == 64 ? 2048 : kUnit * kRowBytes;  // of 64 values the second 16 tokens may lie apart, see half_step
+    static constexpr int kStage = 2 * kPlane, kHeadStage = 2 * kUnit * kHeads * 4;
+    // The row of a group of 8 that stands in row r of an operand.  With it no read of codes has a bank conflict: the eight (16) lanes of a phase
+    // of 16-byte (8-byte) reads meet different banks, for keys (tokens r, r + 1, ...) and for values (every second one).
+    static __device__ __forceinline__ int placed(int r) {
+        return DIM == 128 ? (0x65217430 >> (4 * r)) & 7 : r ^ ((r >> 2) & 1);  // 0 3 4 7 1 2 5 6 and 0 1 2 3 5 4 7 6
+    }
+    // Where byte b of row r < 16 lies in a half of a plane
+    static __device__ __forceinline__ int place(int r, int b) {
+        const int at = r * kRowBytes + b;
+        return at ^ (at >> 3 & 0x70);
+    }
 };
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -105,8 +115,17 @@ __device__ __forceinline__ uint32_t rest_pair(float lo, float hi, uint32_t pair)
 __device__ __forceinline__ float of_bit(int b) { return b == 0 ? 0x1p-14f : b == 1 ? 0x1p-13f : b == 2 ? 0x1p-11f : 0x1p-7f; }
 // Bits 0..3 of x as the bytes of a word
 __device__ __forceinline__ uint32_t bytes_of_bits(uint32_t x) { return (x & 15u) * 0x00204081u & 0x01010101u; }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+// A box of lines of a page (TMA, 128-byte swizzle) and a run of bytes, both counted on an mbarrier.
+__device__ __forceinline__ void load_lines(uint32_t dst, const CUtensorMap* map, int line, uint32_t record, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(0), "r"(line),
+                 "r"(record), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void load_bytes(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// A barrier of `THREADS` threads, which leaves the fetching warp out
+template <int THREADS>
+__device__ __forceinline__ void sync_workers() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
 
 template <int WORDS>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
@@ -135,23 +154,21 @@ template <int DIM, int NB, int WARPS>
 struct Joining {
     static constexpr int kStride = DIM * 18 / 16 + 4;  // rows of 16 values lie 18 apart: no bank conflicts between lanes
     float o[WARPS][8][kStride];
-    float m[8 * NB][WARPS], l[8 * NB][WARPS];  // of the warps; then m is the factor that brings a warp's sums to the row's maximum
-    float top[8 * NB], sum[8 * NB];
+    float m[8 * NB][16], l[8 * NB][16];  // of the warps
     static __device__ __forceinline__ int at(int d) { return d + 2 * (d / 16); }
-};
-// The same memory when the CTAs' parts are joined
-template <int NB>
-struct JoiningCtas {
-    float m[kMostCtas][8 * NB], l[kMostCtas][8 * NB];
 };
 
 template <int DIM, int PARTS, int NB, int WARPS>
 struct Layout {
-    static constexpr int kStages = 2;
-    static constexpr int kQueries = WARPS * kStages * Shape<DIM>::kStage;
+    static constexpr int kStages = DIM == 256 ? 2 : 3, kSlots = WARPS * kStages;
+    static constexpr int kHeads = kSlots * Shape<DIM>::kStage;
+    static constexpr int kQueries = kHeads + kSlots * Shape<DIM>::kHeadStage;
     static constexpr int kJoining = kQueries + (int)sizeof(Queries<DIM, PARTS, NB>);
-    static constexpr int kBytes = kJoining + (int)sizeof(Joining<DIM, NB, WARPS>);
-    static_assert(sizeof(JoiningCtas<NB>) <= sizeof(Joining<DIM, NB, WARPS>::o), "shared memory");
+    static constexpr int kFull = kJoining + (int)sizeof(Joining<DIM, NB, WARPS>), kEmpty = kFull + 8 * kSlots;
+    static constexpr int kThere = kEmpty + 8 * kSlots;  // bit h: the unit's tokens 16 h .. 16 h + 15 have a page
+    static constexpr int kLast = kThere + 4 * kSlots;
+    static constexpr int kBytes = kLast + 16 + 1024;    // and what it takes to begin at a multiple of 1024
+    static_assert(WARPS <= 16, "rows of Joining::m");
 };
 
 // A place in the CTA's row of units: tile `tile` of `tiles` of (seq, head, query tile).
@@ -178,34 +195,6 @@ __device__ __forceinline__ void next_segment(const Attend& a, Place& p) {
     } while (p.qtiles == 0);
 }
 
-// What a warp fetches next: the units of its CTA from `place` on, every WARPS-th of a segment.
-template <int ROWS, int WARPS>
-struct Cursor {
-    Place place;
-    int left = 0;      // units of the CTA from the segment's first one here on
-    int i = 0, n = 0;  // unit in the segment's part that the CTA has, and their number
-    int page[2] = {-1, -1};
-    __device__ __forceinline__ void begin(const Attend& a, const Place& p, int units, int warp) {
-        place = p;
-        left = units;
-        i = warp;
-        n = min(place.tiles - place.tile, left);
-        settle(a, warp);
-    }
-    __device__ __forceinline__ void settle(const Attend& a, int warp) {
-        while (i >= n) {
-            left -= n;
-            if (left <= 0) return;
-            next_segment<ROWS>(a, place);
-            i = warp;
-            n = min(place.tiles, left);
-        }
-        const int token = (place.tile + i) * kUnit;
-        page[0] = page_of(a, place.seq, token, place.s.len);
-        page[1] = page_of(a, place.seq, token + 16, place.s.len);
-    }
-};
-
 // The units' cut: CTA c has base units, and one more where c < more.
 struct Cut {
     int base, more;
@@ -216,30 +205,42 @@ struct Cut {
     }
 };
 
+// A thread's part of a tile of queries on its way to shared memory: blocks of 8 values of rows, whole warps at a time.
 template <int DIM, int PARTS, int NB, int WARPS>
-__device__ __forceinline__ void load_queries(const Attend& a, const Place& p, Queries<DIM, PARTS, NB>& s) {
-    constexpr int kBlocks = DIM / 8;
-    const int rows = min(8 * NB, p.s.count * a.group - p.qtile * 8 * NB);
-    for (int at = threadIdx.x; at < 8 * NB * kBlocks; at += 32 * WARPS) {  // whole warps go round together
-        const int r = at / kBlocks, b = at % kBlocks, row = p.qtile * 8 * NB + r;
-        const int query = row / a.group, q_head = p.head * a.group + row % a.group;
-        float x[8];
+struct QueryBlocks {
+    static constexpr int kBlocks = DIM / 8, kAll = 8 * NB * kBlocks, kRounds = (kAll + 32 * WARPS - 1) / (32 * WARPS);
+    uint4 x[kRounds][PARTS - 1];
+    uint64_t bits[kRounds];
+    __device__ __forceinline__ void load(const Attend& a, const Place& p) {
+        const int rows = min(8 * NB, p.s.count * a.group - p.qtile * 8 * NB);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-        uint64_t bits = 0;
-        if (r < rows) {
-            const int64_t e = (p.s.first + query) * a.q_token_stride + q_head * a.q_head_stride + 8 * b;
-            if (PARTS == 2) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + e));
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        for (int i = 0; i < kRounds; ++i) {
+            const int at = threadIdx.x + i * 32 * WARPS, r = at / kBlocks, b = at % kBlocks;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
-            } else {
-                const float4 v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + e)), w = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + e) + 1);
-                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
+            for (int k = 0; k < PARTS - 1; ++k) x[i][k] = make_uint4(0, 0, 0, 0);
+            bits[i] = 0;
+            if (r < rows) {
+                const int row = p.qtile * 8 * NB + r, query = row / a.group;
+                const int64_t e = (p.s.first + query) * a.q_token_stride + (p.head * a.group + row - query * a.group) * a.q_head_stride + 8 * b;
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + e * (PARTS == 2 ? 2 : 4));
+#pragma unroll
+                for (int k = 0; k < PARTS - 1; ++k) x[i][k] = __ldg(src + k);
+                if (b == 0) bits[i] = a.tree ? (uint64_t)__ldg(a.tree + p.s.first + query) : (uint64_t)query;
             }
-            if (b == 0) bits = a.tree ? (uint64_t)__ldg(a.tree + p.s.first + query) : (uint64_t)query;
         }
+    }
+    __device__ __forceinline__ void put(const Attend& a, Queries<DIM, PARTS, NB>& s) const {
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) {
+            if (threadIdx.x / 32 * 32 + i * 32 * WARPS < kAll) put_one(a, s, threadIdx.x + i * 32 * WARPS, x[i], bits[i]);
+        }
+    }
+    static __device__ __forceinline__ void put_one(const Attend& a, Queries<DIM, PARTS, NB>& s, int at, const uint4 (&raw)[PARTS - 1], uint64_t bits) {
+        const int r = at / kBlocks, b = at % kBlocks;
+        float x[8];
+        const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[PARTS - 2].x, raw[PARTS - 2].y, raw[PARTS - 2].z, raw[PARTS - 2].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = PARTS == 3 ? __uint_as_float(w[i]) : __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
         uint32_t most = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);
@@ -249,179 +250,178 @@ __device__ __forceinline__ void load_queries(const Attend& a, const Place& p, Qu
         constexpr int kTop = 8 * PARTS - 1;
         const bool number = most < 0x7F800000u;
         const int exponent = number ? min(kTop - 1 - ((int)(most >> 23) - 127), 126) : 0;
-        const float up = __uint_as_float((uint32_t)(exponent + 127) << 23);
-        int q[8], total[PARTS], sum = 0;
+        const float up = number ? __uint_as_float((uint32_t)(exponent + 127) << 23) : 0.0f;
+        uint32_t q[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            q[i] = number ? min(__float2int_rn(x[i] * up), (1 << kTop) - 1) : 0;
-            sum += q[i];
-        }
+        for (int i = 0; i < 8; ++i) q[i] = number ? (uint32_t)min(__float2int_rn(x[i] * up), (1 << kTop) - 1) : 0u;
         const int lane = (r % 8) * 4 + b / (DIM / 32), word = b % (DIM / 32);
+        int part_sum[PARTS], sum = 0;
 #pragma unroll
         for (int j = 0; j < PARTS; ++j) {
-            const int shift = 8 * (PARTS - 1 - j);
-            uint32_t even = 0, odd = 0;
-            total[j] = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int part = j == 0 ? q[i] >> shift : q[i] >> shift & 255;
-                total[j] += part;
-                (i & 1 ? odd : even) |= (uint32_t)(part & 255) << (4 * (i & 6));
-            }
+            const int byte = PARTS - 1 - j;  // of q
+            const uint32_t pick = byte * 0x11 + 0x40;
+            const uint32_t even = __byte_perm(__byte_perm(q[0], q[2], pick), __byte_perm(q[4], q[6], pick), 0x5410);
+            const uint32_t odd = __byte_perm(__byte_perm(q[1], q[3], pick), __byte_perm(q[5], q[7], pick), 0x5410);
             s.words[r / 8][j][word][lane] = make_uint2(even, odd);
+            part_sum[j] = j == 0 ? __dp4a((int)even, 0x01010101, __dp4a((int)odd, 0x01010101, 0)) : (int)__dp4a(even, 0x01010101u, __dp4a(odd, 0x01010101u, 0u));
+            sum = sum * 256 + part_sum[j];
+        }
+        // bytes of half the block's sum, four blocks to a word
+        const int half = (sum + 1) >> 1;
 #pragma unroll
-            for (int m = 1; m < kBlocks; m *= 2) total[j] += __shfl_xor_sync(0xFFFFFFFFu, total[j], m);
-            // four neighbours have the bytes of a word of the blocks' sums; with 64 values there are two, and the others are zero
-            const int half = (sum + 1) >> 1, part = j == 0 ? half >> shift : half >> shift & 255;
-            uint32_t low = j == 0 ? part & 63 : part, high = j == 0 ? part >> 6 & 255 : 0;
-            low <<= 8 * (word & 3);
-            high <<= 8 * (word & 3);
+        for (int j = 0; j < PARTS; ++j) {
+            const int part = half >> (8 * (PARTS - 1 - j));
+            uint8_t* at_block = reinterpret_cast<uint8_t*>(&s.blocks[r / 8][j][word / 4][lane]) + (word & 3);
+            at_block[0] = (uint8_t)(j == 0 ? part & 63 : part);
+            at_block[4] = (uint8_t)(j == 0 ? part >> 6 : 0);
+            if (DIM == 64) at_block[2] = at_block[6] = 0;  // a lane has two blocks of 64 values
+        }
+        int total = part_sum[0] * 65536 + part_sum[PARTS - 1];  // both fit 16 bits when summed: |q| < 2^7 and 2^8 in 256 values
+        int middle = PARTS == 3 ? part_sum[1] : 0;
 #pragma unroll
-            for (int m = 1; m < (DIM == 64 ? 2 : 4); m *= 2) {
-                low |= __shfl_xor_sync(0xFFFFFFFFu, low, m);
-                high |= __shfl_xor_sync(0xFFFFFFFFu, high, m);
-            }
-            if ((word & 3) == 0) s.blocks[r / 8][j][word / 4][lane] = make_uint2(low, high);
-            if (b == 0) s.start[j][r] = kExact - 8 * total[j];
+        for (int m = 1; m < kBlocks; m *= 2) {
+            total += __shfl_xor_sync(0xFFFFFFFFu, total, m);
+            if (PARTS == 3) middle += __shfl_xor_sync(0xFFFFFFFFu, middle, m);
         }
         if (b == 0) {
-            s.factor[r] = number ? a.scale * 1.44269504f / up : __uint_as_float(0x7FC00000u);
+            s.start[PARTS - 1][r] = kExact - 8 * (total & 0xFFFF);
+            s.start[0][r] = kExact - 8 * (total >> 16);
+            if (PARTS == 3) s.start[1][r] = kExact - 8 * middle;
+            s.factor[r] = number ? a.scale * 1.44269504f * __uint_as_float((uint32_t)(127 - exponent) << 23) : __uint_as_float(0x7FC00000u);
             s.bits[r] = bits;
         }
     }
-}
+};
 
 template <int DIM, int PARTS, int NB, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, 1)
-k_cache_attend(const __grid_constant__ Attend a) {
+__global__ void __launch_bounds__(32 * WARPS + 32, 1)
+k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtensorMap map) {
     using S = Shape<DIM>;
     using L = Layout<DIM, PARTS, NB, WARPS>;
     constexpr int kRows = 8 * NB, kThreads = 32 * WARPS, kWeights = PARTS - 1;  // 16-bit parts of a weight
     constexpr float kSlack = PARTS == 3 ? 2.0f : 8.0f, kShift = PARTS == 3 ? 12.0f : 6.0f;  // weights reach 2^(1 + kSlack + kShift)
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t scan[WARPS];
-    __shared__ int found_seq, found_before, is_last;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_base = umma::smem_u32(smem_raw), base = (raw_base + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (base - raw_base);
     auto& queries = *reinterpret_cast<Queries<DIM, PARTS, NB>*>(smem + L::kQueries);
     auto& joining = *reinterpret_cast<Joining<DIM, NB, WARPS>*>(smem + L::kJoining);
+    int& is_last = *reinterpret_cast<int*>(smem + L::kLast);
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    if (threadIdx.x < L::kSlots) {
+        umma::mbar_init(base + L::kFull + 8 * threadIdx.x, 1);
+        umma::mbar_init(base + L::kEmpty + 8 * threadIdx.x, 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     grid_wait();
     grid_trigger();
 
-    // ---- this CTA's units
+    // ---- this CTA's units; every warp finds them by itself
+    Place place;
     const auto units_of = [&](int b) {
+        place.s.count = 0;
         if (b >= a.n_seqs) return (int64_t)0;
-        Place p;
-        p.seq = b;
-        enter<kRows>(a, p);
-        return (int64_t)p.qtiles * a.pages.n_heads * p.tiles;
+        place.seq = b;
+        enter<kRows>(a, place);
+        return (int64_t)place.qtiles * a.pages.n_heads * place.tiles;
     };
-    // sum over this and the threads before; *sum: over all of them
-    const auto inclusive = [&](int64_t v, int64_t* sum) {
+    const auto inclusive = [&](int64_t v) {
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
             const int64_t u = __shfl_up_sync(0xFFFFFFFFu, v, d);
             if (lane >= d) v += u;
         }
-        __syncthreads();
-        if (lane == 31) scan[warp] = v;
-        __syncthreads();
-        int64_t mine = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) mine += scan[w];
-            all += scan[w];
-        }
-        *sum = all;
-        return v + mine;
+        return v;
     };
-    if (threadIdx.x == 0) found_seq = -1;
-    int64_t all, units = units_of(threadIdx.x), upto = inclusive(units, &all);
-    const int64_t first_sum = all;
-    for (int b = kThreads; b < a.n_seqs; b += kThreads) {
-        int64_t more;
-        inclusive(units_of(b + threadIdx.x), &more);
-        all += more;
-    }
+    int64_t all = 0;
+    for (int b = 32; b < a.n_seqs; b += 32) all += __shfl_sync(0xFFFFFFFFu, inclusive(units_of(b + lane)), 31);
+    int64_t units = units_of(lane), upto = inclusive(units);
+    all += __shfl_sync(0xFFFFFFFFu, upto, 31);
     if (all < 1 || all > INT32_MAX) return;  // so many only from starts that overlap: the host refuses as much work
     const int total = (int)all, ctas = min((int)gridDim.x, (total - 1) / kLeastUnits + 1);
     if (blockIdx.x >= ctas) return;
     const Cut cut = {total / ctas, total % ctas};
     const int from = cut.from(blockIdx.x), to = cut.from(blockIdx.x + 1);
-    int64_t before = 0, sum = first_sum;
-    for (int b = 0;; before += sum) {
-        if (b > 0) {
-            units = units_of(b + threadIdx.x);
-            upto = inclusive(units, &sum) + before;
+    for (int b = 0;;) {
+        const uint32_t here = __ballot_sync(0xFFFFFFFFu, upto - units <= from && from < upto);
+        if (here || b + 32 >= a.n_seqs) {  // the lane that has this CTA's first unit tells the others
+            const int src = here ? __ffs(here) - 1 : 0, rest = from - (int)__shfl_sync(0xFFFFFFFFu, upto - units, src);
+            place.s.first = __shfl_sync(0xFFFFFFFFu, place.s.first, src);
+            place.s.count = __shfl_sync(0xFFFFFFFFu, place.s.count, src);
+            place.s.len = __shfl_sync(0xFFFFFFFFu, place.s.len, src);
+            place.qtiles = __shfl_sync(0xFFFFFFFFu, place.qtiles, src);
+            place.tiles = __shfl_sync(0xFFFFFFFFu, place.tiles, src);
+            place.seq = b + src;
+            const int segment = rest / place.tiles;
+            place.tile = rest - segment * place.tiles;
+            place.head = segment / place.qtiles;
+            place.qtile = segment - place.head * place.qtiles;
+            break;
         }
-        if (upto - units <= from && from < upto) {
-            found_seq = b + threadIdx.x;
-            found_before = (int)(upto - units);
-        }
-        __syncthreads();
-        b += kThreads;
-        if (found_seq >= 0 || b >= a.n_seqs) break;
+        b += 32;
+        const int64_t before = __shfl_sync(0xFFFFFFFFu, upto, 31);
+        units = units_of(b + lane);
+        upto = before + inclusive(units);
     }
-    Place place;
-    place.seq = found_seq;
-    enter<kRows>(a, place);
-    {
-        const int segment = (from - found_before) / place.tiles;
-        place.tile = (from - found_before) % place.tiles;
-        place.head = segment / place.qtiles;
-        place.qtile = segment % place.qtiles;
-    }
+    QueryBlocks<DIM, PARTS, NB, WARPS> raw;
+    if (warp < WARPS) raw.load(a, place);
+    __syncthreads();  // the barriers are there
+    const int half_step = DIM == 64 && a.pages.page_log2 == 4 ? 1024 : 16 * S::kRowBytes;  // to the second 16 tokens; a swizzled box begins at a multiple of 1024
 
-    // ---- fetching
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * L::kStages * S::kStage;
-    const uint8_t* ring_at = smem + warp * L::kStages * S::kStage;
-    Cursor<kRows, WARPS> cursor;
-    const int page_log2 = a.pages.page_log2, page_mask = (1 << page_log2) - 1;
-    const uint32_t record_chunks = (row_words(DIM) * 4 / 8) << (page_log2 - 1);  // 16-byte chunks; rows are multiples of 8 bytes, pages of 16 rows
-    const uint32_t to_chunk = ring + (lane / S::kChunks) * S::kRowBytes + 16 * S::chunk(lane / S::kChunks, lane % S::kChunks);
-    const uint32_t to_odd_chunk = ring + (lane / S::kChunks) * S::kRowBytes + 16 * S::chunk(lane / S::kChunks + 4, lane % S::kChunks);
-    const uint32_t to_head = ring + 2 * kUnit * S::kRowBytes + ((lane / 16) * kUnit + lane % 16) * S::kHeads * 4;
-    const uint32_t from_head = (2 * S::kRowBytes + (lane / 16) * S::kHeads * 4 << page_log2) + lane % 16 * S::kHeads * 4;
-    // Fetches the next unit; bit h of the result: its tokens 16 h .. 16 h + 15 have a page.
-    const auto fetch = [&](int stage) {
-        int there = 0;
-        if (cursor.left > 0) {
-            const int token = (cursor.place.tile + cursor.i) * kUnit;
+    // ---- the fetching warp: lane w brings the units of warp w
+    if (warp == WARPS) {
+        const bool whole_units = a.pages.page_log2 > 4;
+        const int page_size = 1 << a.pages.page_log2, page_mask = page_size - 1;
+        const uint32_t record_bytes = (uint32_t)(row_words(DIM) * 4) << a.pages.page_log2;
+        const uint8_t* pages = reinterpret_cast<const uint8_t*>(a.pages.words);
+        int count = 0;
+        bool lost = false;
+        for (int unit = from; unit < to;) {
+            const int n = min(place.tiles - place.tile, to - unit);
+            for (int i = lane; i < n + lane; i += WARPS) {
+                if (lane < WARPS && i < n && !lost) {
+                    const int token = (place.tile + i) * kUnit, row = token & page_mask, slot = lane * L::kStages + count % L::kStages;
+                    const int page0 = page_of(a, place.seq, token, place.s.len), page1 = whole_units ? -1 : page_of(a, place.seq, token + 16, place.s.len);
+                    if (count >= L::kStages) lost = !umma::mbar_wait(base + L::kEmpty + 8 * slot, (count / L::kStages - 1) & 1);
+                    const uint32_t full = base + L::kFull + 8 * slot, to_codes = base + slot * S::kStage, to_heads = base + L::kHeads + slot * S::kHeadStage;
+                    const int run = whole_units ? kUnit : 16;  // tokens of a copy
+                    const int there = whole_units ? (page0 >= 0 ? 3 : 0) : (page0 >= 0 ? 1 : 0) + (page1 >= 0 ? 2 : 0);
+                    if (!lost) {
+                        *reinterpret_cast<int*>(smem + L::kThere + 4 * slot) = there;
+                        umma::mbar_arrive_expect_tx(full, __popc(there) * 16 * (2 * S::kRowBytes + 2 * S::kHeads * 4));
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int page = cursor.page[h];
-                if (page < 0) continue;
-                there |= 1 << h;
-                const uint64_t chunk = ((uint64_t)(uint32_t)page * (uint32_t)a.pages.n_heads + (uint32_t)cursor.place.head) * record_chunks;
-                const uint8_t* rec = reinterpret_cast<const uint8_t*>(a.pages.words) + chunk * 16;
-                const uint32_t row0 = (uint32_t)(token + 16 * h) & page_mask;
-                const uint8_t* key = rec + row0 * S::kRowBytes + lane * 16;
-                const uint8_t* value = key + ((uint32_t)S::kRowBytes << page_log2);
-                const uint8_t* head = rec + row0 * S::kHeads * 4 + from_head;
-                const uint32_t dst = stage * S::kStage + 16 * h * S::kRowBytes;
-#pragma unroll
-                for (int i = 0; i < S::kRowBytes / 32; ++i) {  // 32 chunks, 32 / kChunks rows at a time
-                    const uint32_t at = (DIM == 256 && (i & 1) ? to_odd_chunk : to_chunk) + dst + i * 512;  // four rows of 256 further the swizzle differs
-                    copy16(at, key + i * 512);
-                    copy16(at + kUnit * S::kRowBytes, value + i * 512);
+                        for (int h = 0; h < 2; ++h) {
+                            const int page = h == 0 ? page0 : page1, row0 = h == 0 ? row : 0;  // pages of 16 tokens begin with the half
+                            if (page < 0) continue;
+                            const uint32_t rec = (uint32_t)page * (uint32_t)a.pages.n_heads + (uint32_t)place.head;
+                            load_lines(to_codes + h * half_step, &map, row0 * S::kRowBytes / 128, rec, full);
+                            load_lines(to_codes + S::kPlane + h * half_step, &map, (page_size + row0) * S::kRowBytes / 128, rec, full);
+                            const uint8_t* heads = pages + (uint64_t)rec * record_bytes + (((uint32_t)(2 * S::kRowBytes) << a.pages.page_log2) + row0 * S::kHeads * 4);
+                            load_bytes(to_heads + h * 16 * S::kHeads * 4, heads, run * S::kHeads * 4, full);
+                            load_bytes(to_heads + (kUnit + h * 16) * S::kHeads * 4, heads + (S::kHeads * 4 << a.pages.page_log2), run * S::kHeads * 4, full);
+                        }
+                    }
+                    ++count;
                 }
-#pragma unroll
-                for (int i = 0; i < S::kHeads; ++i) copy4(to_head + stage * S::kStage + (16 * h * S::kHeads + i) * 4, head + 4 * i);
+                __syncwarp();
             }
-            cursor.i += WARPS;
-            cursor.settle(a, warp);
+            unit += n;
+            next_segment<kRows>(a, place);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        return there;
-    };
-    cursor.begin(a, place, to - from, warp);
-    int stage = 0, there = fetch(0);
+        return;
+    }
+    // where a lane reads in a stage: keys of token g, values of tokens 2 t and 2 t + 1, and their heads
+    const int key_at = S::place(S::placed(g), t * (DIM / 8)), key_at_1 = S::place(S::placed(g), t * (DIM / 8) + 16);  // of 256 values, the second half
+    const int value_at = S::kPlane + S::place(S::placed(2 * t), g * (DIM / 16)), value_at_1 = S::kPlane + S::place(S::placed(2 * t + 1), g * (DIM / 16));
+    const int head_at = S::placed(g) * S::kHeads * 4;
+    const int pair_at = (kUnit + S::placed(2 * t)) * S::kHeads * 4 + (DIM == 256 ? g / 4 * 4 : 0), pair_at_1 = (kUnit + S::placed(2 * t + 1)) * S::kHeads * 4 + (DIM == 256 ? g / 4 * 4 : 0);
+    int stage = 0, phase = 0;
+    bool lost = false;  // a wait gave up: results are not numbers
 
     // ---- one (sequence, head, tile of queries) after the other
     for (int unit = from; unit < to;) {
         const int n = min(place.tiles - place.tile, to - unit);
-        __syncthreads();  // nobody reads the queries before, nor joins any more
-        load_queries<DIM, PARTS, NB, WARPS>(a, place, queries);
-        __syncthreads();
+        raw.put(a, queries);
+        sync_workers<kThreads>();
         float o[NB][S::kTiles][4], bits[NB][S::kBitTiles][4], m[NB][2], l[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -437,13 +437,14 @@ k_cache_attend(const __grid_constant__ Attend a) {
         }
         const int drafted = place.s.len - place.s.count;
         for (int i = warp; i < n; i += WARPS) {
-            __syncwarp();  // every lane has read the stage that is filled next
-            const int there_next = fetch(stage ^ 1);
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            __syncwarp();
-            const uint8_t* at = ring_at + stage * S::kStage;
-            const uint32_t* key_heads = reinterpret_cast<const uint32_t*>(at + 2 * kUnit * S::kRowBytes);
-            const uint32_t* value_heads = key_heads + kUnit * S::kHeads;
+            const int slot = warp * L::kStages + stage;
+            if (lost || !umma::mbar_wait_warp(base + L::kFull + 8 * slot, phase)) {
+                lost = true;
+                break;
+            }
+            const uint8_t *at = smem + slot * S::kStage, *heads = smem + L::kHeads + slot * S::kHeadStage;
+            const int there = *reinterpret_cast<const int*>(smem + L::kThere + 4 * slot);
+            const auto head_word = [&](int byte) { return *reinterpret_cast<const uint32_t*>(heads + byte); };
             const int token0 = (place.tile + i) * kUnit;
 
             // scores: [group of 16 tokens][tile of 8 queries][token g: query 2 t, 2 t + 1; token g + 8: the same]
@@ -462,15 +463,12 @@ k_cache_attend(const __grid_constant__ Attend a) {
                 uint32_t kw[2][S::kKeyWords], kh[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int r = 16 * h + 8 * e + placed(g);
-                    const uint8_t* row = at + r * S::kRowBytes;
-                    if (DIM == 64) {
-                        load_words<2>(row + 8 * t, kw[e]);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < S::kKeyWords / 4; ++c) load_words<4>(row + 16 * S::chunk(r, t * (S::kKeyWords / 4) + c), kw[e] + c * 4);
-                    }
-                    kh[e] = key_heads[r * S::kHeads + (DIM == 256 ? t / 2 : 0)];
+                    // eight rows of 64 (128, 256) values are 256 (512, 1024) bytes, and the swizzle turns with every 1024
+                    const int rows = h * half_step + 8 * e * S::kRowBytes, turn = DIM == 64 ? (h * (half_step >> 3 & 0x40) + 0x20 * e) : DIM == 128 ? 0x40 * e : 0;
+                    if (DIM == 64) load_words<2>(at + ((key_at ^ turn) + rows), kw[e]);
+                    else load_words<4>(at + ((key_at ^ turn) + rows), kw[e]);
+                    if (DIM == 256) load_words<4>(at + (key_at_1 + rows), kw[e] + S::kKeyWords / 2);
+                    kh[e] = head_word(head_at + (16 * h + 8 * e) * S::kHeads * 4 + (DIM == 256 ? t / 2 * 4 : 0));
                     step[h][e] = __uint_as_float(kh[e] & 0xFFFF0000u);
                 }
 #pragma unroll
@@ -525,7 +523,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
                             for (int h = 0; h < 2; ++h)
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
-                                    const int token = token0 + 16 * h + 8 * e + placed(g), j = token - drafted;
+                                    const int token = token0 + 16 * h + 8 * e + S::placed(g), j = token - drafted;
                                     const bool yes = token < place.s.len && (there >> h & 1) &&
                                                      (j < 0 || (a.tree ? j < 64 && (who >> j & 1) : j <= (int)who));
                                     seen[nb] |= (uint32_t)yes << (4 * h + 2 * e + c);
@@ -539,7 +537,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const uint32_t v = value_heads[(16 * h + 8 * e + placed(g)) * S::kHeads];
+                        const uint32_t v = head_word(head_at + (kUnit + 16 * h + 8 * e) * S::kHeads * 4);
                         value_step[h][e] = __uint_as_float(v & 0xFFFF0000u);
                         size[h][e] = fmaxf(__uint_as_float(0x4B400000u + (v >> 23 & 255u)) - (kExactly + 127.0f), (float)kLeastSize);
                     }
@@ -606,11 +604,9 @@ k_cache_attend(const __grid_constant__ Attend a) {
                 uint32_t vw[4][S::kValueWords], vh[4];  // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int r = 16 * h + 8 * (k >> 1) + placed(2 * t + (k & 1));
-                    const uint8_t* row = at + (kUnit + r) * S::kRowBytes;
-                    const int byte = g * (DIM / 16);
-                    load_words<S::kValueWords>(row + 16 * S::chunk(r, byte / 16) + byte % 16, vw[k]);
-                    vh[k] = value_heads[r * S::kHeads + (DIM == 256 ? g / 4 : 0)];
+                    const int e = k >> 1, rows = h * half_step + 8 * e * S::kRowBytes, turn = DIM == 64 ? (h * (half_step >> 3 & 0x40) + 0x20 * e) : DIM == 128 ? 0x40 * e : 0;
+                    load_words<S::kValueWords>(at + (((k & 1 ? value_at_1 : value_at) ^ turn) + rows), vw[k]);
+                    vh[k] = head_word((k & 1 ? pair_at_1 : pair_at) + (16 * h + 8 * e) * S::kHeads * 4);
                 }
                 const auto add = [&](float (&acc)[NB][S::kTiles][4], int tile, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
@@ -637,8 +633,16 @@ k_cache_attend(const __grid_constant__ Attend a) {
                             mma(bits[nb][k], x & (0x04000400u << (2 * k)), x & (0x08000800u << (2 * k)), y & (0x04000400u << (2 * k)), y & (0x08000800u << (2 * k)),
                                 p[h][nb][0][part], p[h][nb][1][part]);
             }
-            stage ^= 1;
-            there = there_next;
+            __syncwarp();  // every lane has read
+            if (lane == 0) umma::mbar_arrive(base + L::kEmpty + 8 * slot);
+            if (++stage == L::kStages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+        if (lost) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = __uint_as_float(0x7FC00000u);
         }
 
         // ---- the warps' parts into one
@@ -656,19 +660,17 @@ k_cache_attend(const __grid_constant__ Attend a) {
                     joining.l[8 * nb + 2 * t + c][warp] = x;
                 }
             }
-        __syncthreads();
-        if (threadIdx.x < kRows) {
-            float top = -INFINITY, sum = 0.0f;
-            for (int w = 0; w < live; ++w) top = larger(top, joining.m[threadIdx.x][w]);
-            for (int w = 0; w < live; ++w) {
-                const float its = joining.m[threadIdx.x][w], keep = its == -INFINITY ? 0.0f : exp2_of(its - top);
-                joining.m[threadIdx.x][w] = keep;
-                if (keep != 0.0f) sum += joining.l[threadIdx.x][w] * keep;
-            }
-            joining.top[threadIdx.x] = top;
-            joining.sum[threadIdx.x] = sum;
-        }
-        __syncthreads();
+        Place next = place;
+        next_segment<kRows>(a, next);
+        if (unit + n < to) raw.load(a, next);  // the next tile's queries, on their way meanwhile
+        sync_workers<kThreads>();
+        // of row r: the largest maximum of the warps
+        const auto top_of = [&](int r) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) top = w < live ? larger(top, joining.m[r][w]) : top;
+            return top;
+        };
         const int q_heads = a.group * a.pages.n_heads;
         // row r of the tile: where its result goes
         const auto row_of = [&](int r) {
@@ -687,11 +689,11 @@ k_cache_attend(const __grid_constant__ Attend a) {
         float* partial = a.partials + ((int64_t)blockIdx.x * 2 + (place.tile > 0 ? 0 : 1)) * kPart;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            if (nb > 0) __syncthreads();  // the tile before is read
+            if (nb > 0) sync_workers<kThreads>();  // the tile before is read
             if (warp < live) {
                 float scale[2];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) scale[c] = joining.m[8 * nb + 2 * t + c][warp];
+                for (int c = 0; c < 2; ++c) scale[c] = m[nb][c] == -INFINITY ? 0.0f : exp2_of(m[nb][c] - top_of(8 * nb + 2 * t + c));
 #pragma unroll
                 for (int k = 0; k < S::kTiles; ++k) {
                     const int d = g * (DIM / 8) + 2 * k, block = k / 4;  // of the lane's blocks
@@ -704,17 +706,22 @@ k_cache_attend(const __grid_constant__ Attend a) {
                     }
                 }
             }
-            __syncthreads();
+            sync_workers<kThreads>();
             for (int at = threadIdx.x; at < 8 * DIM / 2; at += kThreads) {
                 const int r = 8 * nb + at / (DIM / 2), d = at % (DIM / 2) * 2;
                 if (r >= rows) continue;
                 float2 v = make_float2(0.0f, 0.0f);
-                for (int w = 0; w < live; ++w) {
+                const float top = top_of(r);
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) {
+                    if (w >= live) break;
                     const float2 x = *reinterpret_cast<const float2*>(&joining.o[w][r % 8][joining.at(d)]);
                     v.x += x.x;
                     v.y += x.y;
+                    const float its = joining.m[r][w], keep = its == -INFINITY ? 0.0f : exp2_of(its - top);
+                    if (keep != 0.0f) sum += joining.l[r][w] * keep;
                 }
-                const float top = joining.top[r], sum = joining.sum[r];
                 if (whole) {
                     put(r, d, top == -INFINITY ? 0.0f : v.x / sum, top == -INFINITY ? 0.0f : v.y / sum);
                     if (d == 0) put_lse(r, top, sum);
@@ -728,84 +735,98 @@ k_cache_attend(const __grid_constant__ Attend a) {
             }
         }
         // ---- the CTAs' parts into one: those from the CTA with the segment's first unit to the one with its last
+        sync_workers<kThreads>();  // joined, and the parts written
         if (!whole) {
             const int first_cta = cut.cta_of(unit - place.tile), parts = cut.cta_of(unit - place.tile + place.tiles - 1) - first_cta + 1;
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) is_last = atomicAdd(a.counters + first_cta, 1u) == (uint32_t)(parts - 1);
-            __syncthreads();
+            if (threadIdx.x == 0) {
+                uint32_t arrived;
+                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(arrived) : "l"(a.counters + first_cta) : "memory");
+                is_last = arrived == (uint32_t)(parts - 1);
+            }
+            sync_workers<kThreads>();
             if (is_last) {
-                __threadfence();
-                auto& ctas_parts = *reinterpret_cast<JoiningCtas<NB>*>(joining.o);
-                const auto part = [&](int i) { return a.partials + ((int64_t)(first_cta + i) * 2 + (i == 0 ? 1 : 0)) * kPart; };
-                for (int at = threadIdx.x; at < parts * kRows; at += kThreads) {
-                    const int i = at / kRows, r = at % kRows;
-                    ctas_parts.m[i][r] = __ldcg(part(i) + r);
-                    ctas_parts.l[i][r] = __ldcg(part(i) + kRows + r);
-                }
-                __syncthreads();
-                for (int r = warp; r < rows; r += WARPS) {
+                constexpr int kAtOnce = 10;
+                for (int at = threadIdx.x; at < rows * (DIM / 4); at += kThreads) {
+                    const int r = at / (DIM / 4), d = at % (DIM / 4) * 4;
                     float top = -INFINITY, sum = 0.0f;
-                    for (int i = lane; i < parts; i += 32) top = larger(top, ctas_parts.m[i][r]);
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int i0 = 0; i0 < parts; i0 += kAtOnce) {
+                        float m_of[kAtOnce], l_of[kAtOnce];
+                        float4 x[kAtOnce];
 #pragma unroll
-                    for (int d = 1; d < 32; d *= 2) top = larger(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-                    for (int i = lane; i < parts; i += 32) {
-                        const float its = ctas_parts.m[i][r], keep = its == -INFINITY ? 0.0f : exp2_of(its - top);
-                        ctas_parts.m[i][r] = keep;
-                        if (keep != 0.0f) sum += ctas_parts.l[i][r] * keep;
-                    }
+                        for (int i = 0; i < kAtOnce; ++i) {
+                            const float* part = a.partials + ((int64_t)(first_cta + i0 + i) * 2 + (i0 + i == 0 ? 1 : 0)) * kPart;
+                            m_of[i] = -INFINITY;
+                            if (i0 + i < parts) {
+                                m_of[i] = __ldcg(part + r);
+                                l_of[i] = __ldcg(part + kRows + r);
+                                x[i] = __ldcg(reinterpret_cast<const float4*>(part + 2 * kRows + r * DIM + d));
+                            }
+                        }
+                        float higher = top;
 #pragma unroll
-                    for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-                    if (lane == 0) {
-                        joining.top[r] = top;
-                        joining.sum[r] = sum;
-                    }
-                }
-                __syncthreads();
-                for (int at = threadIdx.x; at < rows * (DIM / 2); at += kThreads) {
-                    const int r = at / (DIM / 2), d = at % (DIM / 2) * 2;
-                    float2 v = make_float2(0.0f, 0.0f);
-#pragma unroll 8
-                    for (int i = 0; i < parts; ++i) {
-                        const float2 x = __ldcg(reinterpret_cast<const float2*>(part(i) + 2 * kRows + r * DIM + d));
-                        const float keep = ctas_parts.m[i][r];
-                        if (keep != 0.0f) {
-                            v.x += x.x * keep;
-                            v.y += x.y * keep;
+                        for (int i = 0; i < kAtOnce; ++i) higher = larger(higher, m_of[i]);
+                        const float before = top == -INFINITY ? 0.0f : exp2_of(top - higher);
+                        v.x *= before; v.y *= before; v.z *= before; v.w *= before;
+                        sum *= before;
+                        top = higher;
+#pragma unroll
+                        for (int i = 0; i < kAtOnce; ++i) {
+                            const float keep = m_of[i] == -INFINITY ? 0.0f : exp2_of(m_of[i] - top);
+                            if (keep != 0.0f) {
+                                v.x += x[i].x * keep; v.y += x[i].y * keep; v.z += x[i].z * keep; v.w += x[i].w * keep;
+                                sum += l_of[i] * keep;
+                            }
                         }
                     }
-                    const float top = joining.top[r], sum = joining.sum[r];
-                    put(r, d, top == -INFINITY ? 0.0f : v.x / sum, top == -INFINITY ? 0.0f : v.y / sum);
+                    const float part_of = top == -INFINITY ? 0.0f : 1.0f / sum;
+                    put(r, d, v.x * part_of, v.y * part_of);
+                    put(r, d + 2, v.z * part_of, v.w * part_of);
                     if (d == 0) put_lse(r, top, sum);
                 }
                 if (threadIdx.x == 0) a.counters[first_cta] = 0;
             }
         }
         unit += n;
-        next_segment<kRows>(a, place);
+        place = next;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (lost) {  // what was on its way when the wait gave up has to land before the memory is another's
+        for (int i = 0; i < L::kStages; ++i) umma::mbar_wait_warp(base + L::kFull + 8 * (warp * L::kStages + i), phase);
+    }
 }
 
 constexpr int kMostRows = 16;
 int64_t scratch_bytes_of(int head_dim) { return 4 * kMostCtas + (int64_t)kMostCtas * 2 * kMostRows * (head_dim + 2) * 4; }
 
+// The codes of all records as lines of 128 bytes, [n_records][keys and values]
+template <int DIM>
+int make_map(const Attend& a, CUtensorMap* map) {
+    memset(map, 0, sizeof(*map));
+    if (a.pages.n_pages == 0) return 0;  // nothing is fetched
+    const uint64_t page = 1ull << a.pages.page_log2, record_bytes = page * row_words(DIM) * 4;
+    const cuuint64_t dims[3] = {128, 2 * page * Shape<DIM>::kRowBytes / 128, (cuuint64_t)a.pages.n_pages * a.pages.n_heads}, strides[2] = {128, record_bytes};
+    const cuuint32_t box[3] = {128, (cuuint32_t)(Shape<DIM>::kLines * (a.pages.page_log2 > 4 ? 2 : 1)), 1}, step[3] = {1, 1, 1};
+    return umma::encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.pages.words, dims, strides, box, step);
+}
+
 template <int DIM, int PARTS, int NB, int WARPS>
 int launch_as(const Attend& a, cudaStream_t st) {
     using L = Layout<DIM, PARTS, NB, WARPS>;
-    static_assert(L::kBytes <= 227 * 1024 - 1024, "shared memory");
+    static_assert(L::kBytes <= 227 * 1024, "shared memory");
     static_assert(8 * NB <= kMostRows, "scratch memory");
     const auto kernel = k_cache_attend<DIM, PARTS, NB, WARPS>;
+    CUtensorMap map;
+    if (int e = make_map<DIM>(a, &map)) return e;
     if (int e = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes), "cudaFuncSetAttribute")) return e;
     const int sms = sm_count(), grid = sms < kMostCtas ? sms : kMostCtas;
-    return launch_dependent("e8_cache_attention", kernel, (unsigned)grid, 32 * WARPS, L::kBytes, st, a);
+    return launch_dependent("e8_cache_attention", kernel, (unsigned)grid, 32 * WARPS + 32, L::kBytes, st, a, map);
 }
 
 template <int DIM, int PARTS>
 int launch(const Attend& a, cudaStream_t st) {
     const int64_t rows = ((int64_t)a.n_queries + a.n_seqs - 1) / a.n_seqs * a.group;  // of a cache head, on average
-    if (rows <= 8) return launch_as<DIM, PARTS, 1, DIM == 256 ? 8 : 16>(a, st);
-    return launch_as<DIM, PARTS, 2, DIM == 256 && PARTS == 3 ? 6 : 8>(a, st);
+    if (rows <= 8) return launch_as<DIM, PARTS, 1, DIM == 256 ? 7 : 11>(a, st);
+    return launch_as<DIM, PARTS, 2, 7>(a, st);
 }
 
 }  // namespace
@@ -832,6 +853,7 @@ int coset_e8_cache_attention(const void* q, int dtype, int64_t q_token_stride, i
     if (n_seqs == 0) return 0;
     // no more than this many units are cut among the CTAs, however the queries are shared among the sequences
     const int64_t tiles = ((int64_t)n_queries * (q_heads / n_heads) + 7) / 8 + n_seqs, longest = ((int64_t)max_pages * page_size + kUnit - 1) / kUnit + 1;
+    if (n_pages * n_heads >= UINT32_MAX) return fail(COSET_E_UNSUPPORTED, "2^32 or more records");
     if ((double)tiles * n_heads * longest > 2e9) return fail(COSET_E_UNSUPPORTED, "too much work for one call: queries x pages of the table");
     const int64_t whole = dtype == COSET_DTYPE_F32 ? 4 : 8;
     if (!aligned(q, 16) || !aligned(out, 16) || (q_token_stride | q_head_stride) % whole) return fail(COSET_E_ALIGN, "rows of q and out must be 16-byte aligned");
