@@ -18,14 +18,13 @@
 //
 // Work is cut into units of 32 tokens of one (sequence, head, tile of queries), and the units of all of them in a row are cut evenly among the CTAs, one
 // per SM; the lengths are read on the device, so a captured launch follows them.  A warp runs through its units alone, with the running maximum
-// and sum of the softmax in registers; one more warp, a lane for each of the others, looks up pages and brings the next units' codes by TMA (128-byte
-// swizzle), so that the addresses cost the others nothing.  The warps of a CTA are joined in shared memory, and where several CTAs share a row the last one
-// to arrive joins them in the order of the CTAs.
+// and sum of the softmax in registers and the next units' codes on their way to shared memory (its lanes look up the pages of 32 units at a time, so that
+// addresses cost little); the warps of a CTA are joined in shared memory, and where several CTAs share a row the last one to arrive joins them in the
+// order of the CTAs.
 //
 // The running maximum is that of a weight times the size of its value (s + the exponent of the value's step), so that w = p step fits 16 bits: what is
 // lost is below 2^-31 of the row's largest.  It follows only when it lags by 2^kSlack.  For float32 queries w is split into two 16-bit numbers.
 #include "e8_cache_attention.cuh"
-#include "umma.cuh"
 
 using namespace coset;
 using namespace coset::cache;
@@ -39,26 +38,22 @@ constexpr int kMostCtas = 152;    // counters in the scratch memory
 constexpr int kExact = 0x4B400000;  // the bits of kExactly = 1.5 2^23; a whole number of up to 22 bits added to them is added to it
 constexpr float kExactly = 12582912.0f;
 
-// A unit in shared memory: keys, values (lines of 128 bytes as they are in a page, one or several rows each, swizzled), their heads apart.
+// The row of a group of 8 that stands in row r of an operand: 0 1 2 3 5 4 7 6.  With the swizzle below no read of codes has a bank conflict.
+__device__ __forceinline__ int placed(int r) { return r ^ ((r >> 2) & 1); }
+
+// A unit in shared memory: keys, values, heads of keys, heads of values
 template <int DIM>
 struct Shape {
-    static constexpr int kRowBytes = DIM / 2, kHeads = head_words(DIM);
+    static constexpr int kRowBytes = DIM / 2, kChunks = kRowBytes / 16, kHeads = head_words(DIM);
     static constexpr int kKeyWords = DIM / 32;    // words of a row that a lane has for S
     static constexpr int kValueWords = DIM / 64;  // for O
     static constexpr int kTiles = DIM / 16;       // of O^T
     static constexpr int kBitTiles = DIM == 256 ? 2 : 1;  // of the blocks' bits, for S and for O
-    static constexpr int kLines = 16 * kRowBytes / 128;   // of 16 tokens
-    static constexpr int kPlane = DIM == 64 ? 2048 : kUnit * kRowBytes;  // of 64 values the second 16 tokens may lie apart, see half_step
-    static constexpr int kStage = 2 * kPlane, kHeadStage = 2 * kUnit * kHeads * 4;
-    // The row of a group of 8 that stands in row r of an operand.  With it no read of codes has a bank conflict: the eight (16) lanes of a phase
-    // of 16-byte (8-byte) reads meet different banks, for keys (tokens r, r + 1, ...) and for values (every second one).
-    static __device__ __forceinline__ int placed(int r) {
-        return DIM == 128 ? (0x65217430 >> (4 * r)) & 7 : r ^ ((r >> 2) & 1);  // 0 3 4 7 1 2 5 6 and 0 1 2 3 5 4 7 6
-    }
-    // Where byte b of row r < 16 lies in a half of a plane
+    static constexpr int kPlane = kUnit * kRowBytes, kHeadsAt = 2 * kPlane, kStage = kHeadsAt + 2 * kUnit * kHeads * 4;
+    // Where byte b of row r lies in a plane: 16-byte chunks of rows of 64 (128) bytes are turned by bits of the row, the same ones in every group of 8
     static __device__ __forceinline__ int place(int r, int b) {
-        const int at = r * kRowBytes + b;
-        return at ^ (at >> 3 & 0x70);
+        const int turn = DIM == 64 ? 0 : DIM == 128 ? r & 2 : r & 7;
+        return r * kRowBytes + ((b / 16 ^ turn) * 16 | b % 16);
     }
 };
 
@@ -76,17 +71,30 @@ __device__ __forceinline__ void mma_bytes(int (&c)[4], uint32_t a0, uint32_t a1,
         asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// f = n - 8 of the nibbles at bits 0..3 (even) or 4..7 (odd) of both halves of x, as 16-bit numbers
-__device__ __forceinline__ uint32_t even_values(uint32_t x) {
-    uint32_t d;
-    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"((x & 0x000F000Fu) | 0x64006400u), "r"(0xE408E408u));
-    return d;
-}
-__device__ __forceinline__ uint32_t odd_values(uint32_t x) {
-    uint32_t d;
-    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"((x & 0x00F000F0u) | 0x54005400u), "r"(0xD480D480u));
-    return d;
-}
+// f = n - 8 of the nibbles at bits 0..3 (even) or 4..7 (odd) of both halves of x, as 16-bit numbers.  The compiler makes two instructions of masking and
+// setting the exponent when it knows both constants (120 of them in a unit), hence the registers whose contents it does not know, and the instruction by its name.
+struct Exponents {
+    uint32_t even, odd;  // of 1024 and of 64
+    __device__ __forceinline__ Exponents() {
+        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(even));
+        asm volatile("mov.b32 %0, 0x54005400;" : "=r"(odd));
+    }
+    static __device__ __forceinline__ uint32_t chosen(uint32_t x, uint32_t mask, uint32_t exponent) {
+        uint32_t d;
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "r"(mask), "r"(exponent));  // (x & mask) | exponent
+        return d;
+    }
+    __device__ __forceinline__ uint32_t even_values(uint32_t x) const {
+        uint32_t d;
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(chosen(x, 0x000F000Fu, even)), "r"(0xE408E408u));
+        return d;
+    }
+    __device__ __forceinline__ uint32_t odd_values(uint32_t x) const {
+        uint32_t d;
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(chosen(x, 0x00F000F0u, odd)), "r"(0xD480D480u));
+        return d;
+    }
+};
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
     uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -115,17 +123,8 @@ __device__ __forceinline__ uint32_t rest_pair(float lo, float hi, uint32_t pair)
 __device__ __forceinline__ float of_bit(int b) { return b == 0 ? 0x1p-14f : b == 1 ? 0x1p-13f : b == 2 ? 0x1p-11f : 0x1p-7f; }
 // Bits 0..3 of x as the bytes of a word
 __device__ __forceinline__ uint32_t bytes_of_bits(uint32_t x) { return (x & 15u) * 0x00204081u & 0x01010101u; }
-// A box of lines of a page (TMA, 128-byte swizzle) and a run of bytes, both counted on an mbarrier.
-__device__ __forceinline__ void load_lines(uint32_t dst, const CUtensorMap* map, int line, uint32_t record, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(0), "r"(line),
-                 "r"(record), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void load_bytes(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-// A barrier of `THREADS` threads, which leaves the fetching warp out
-template <int THREADS>
-__device__ __forceinline__ void sync_workers() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
 
 template <int WORDS>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
@@ -158,24 +157,21 @@ struct Joining {
     static __device__ __forceinline__ int at(int d) { return d + 2 * (d / 16); }
 };
 
-template <int DIM, int PARTS, int NB, int WARPS>
-struct Layout {
-    static constexpr int kStages = DIM == 256 ? 2 : 3, kSlots = WARPS * kStages;
-    static constexpr int kHeads = kSlots * Shape<DIM>::kStage;
-    static constexpr int kQueries = kHeads + kSlots * Shape<DIM>::kHeadStage;
-    static constexpr int kJoining = kQueries + (int)sizeof(Queries<DIM, PARTS, NB>);
-    static constexpr int kFull = kJoining + (int)sizeof(Joining<DIM, NB, WARPS>), kEmpty = kFull + 8 * kSlots;
-    static constexpr int kThere = kEmpty + 8 * kSlots;  // bit h: the unit's tokens 16 h .. 16 h + 15 have a page
-    static constexpr int kLast = kThere + 4 * kSlots;
-    static constexpr int kBytes = kLast + 16 + 1024;    // and what it takes to begin at a multiple of 1024
-    static_assert(WARPS <= 16, "rows of Joining::m");
-};
-
 // A place in the CTA's row of units: tile `tile` of `tiles` of (seq, head, query tile).
 struct Place {
     Sequence s;
     int seq, head, qtile, qtiles, tile, tiles;
 };
+template <int DIM, int PARTS, int NB, int WARPS>
+struct Layout {
+    static constexpr int kStages = WARPS > 12 || DIM == 256 ? 2 : 3;
+    static constexpr int kQueries = WARPS * kStages * Shape<DIM>::kStage;
+    static constexpr int kJoining = kQueries + (int)sizeof(Queries<DIM, PARTS, NB>);
+    static constexpr int kLast = kJoining + (int)sizeof(Joining<DIM, NB, WARPS>);
+    static constexpr int kBytes = kLast + 16;
+    static_assert(WARPS <= 16, "rows of Joining::m");
+};
+
 template <int ROWS>
 __device__ __forceinline__ void enter(const Attend& a, Place& p) {
     p.s = sequence(a, p.seq);
@@ -294,24 +290,17 @@ struct QueryBlocks {
 };
 
 template <int DIM, int PARTS, int NB, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS + 32, 1)
-k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtensorMap map) {
+__global__ void __launch_bounds__(32 * WARPS, 1)
+k_cache_attend(const __grid_constant__ Attend a) {
     using S = Shape<DIM>;
     using L = Layout<DIM, PARTS, NB, WARPS>;
     constexpr int kRows = 8 * NB, kThreads = 32 * WARPS, kWeights = PARTS - 1;  // 16-bit parts of a weight
     constexpr float kSlack = PARTS == 3 ? 2.0f : 8.0f, kShift = PARTS == 3 ? 12.0f : 6.0f;  // weights reach 2^(1 + kSlack + kShift)
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t raw_base = umma::smem_u32(smem_raw), base = (raw_base + 1023u) & ~1023u;
-    uint8_t* smem = smem_raw + (base - raw_base);
+    extern __shared__ __align__(128) uint8_t smem[];
     auto& queries = *reinterpret_cast<Queries<DIM, PARTS, NB>*>(smem + L::kQueries);
     auto& joining = *reinterpret_cast<Joining<DIM, NB, WARPS>*>(smem + L::kJoining);
     int& is_last = *reinterpret_cast<int*>(smem + L::kLast);
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    if (threadIdx.x < L::kSlots) {
-        umma::mbar_init(base + L::kFull + 8 * threadIdx.x, 1);
-        umma::mbar_init(base + L::kEmpty + 8 * threadIdx.x, 1);
-    }
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     grid_wait();
     grid_trigger();
 
@@ -363,65 +352,77 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
         upto = before + inclusive(units);
     }
     QueryBlocks<DIM, PARTS, NB, WARPS> raw;
-    if (warp < WARPS) raw.load(a, place);
-    __syncthreads();  // the barriers are there
-    const int half_step = DIM == 64 && a.pages.page_log2 == 4 ? 1024 : 16 * S::kRowBytes;  // to the second 16 tokens; a swizzled box begins at a multiple of 1024
+    raw.load(a, place);
 
-    // ---- the fetching warp: lane w brings the units of warp w
-    if (warp == WARPS) {
-        const bool whole_units = a.pages.page_log2 > 4;
-        const int page_size = 1 << a.pages.page_log2, page_mask = page_size - 1;
-        const uint32_t record_bytes = (uint32_t)(row_words(DIM) * 4) << a.pages.page_log2;
-        const uint8_t* pages = reinterpret_cast<const uint8_t*>(a.pages.words);
-        int count = 0;
-        bool lost = false;
-        for (int unit = from; unit < to;) {
-            const int n = min(place.tiles - place.tile, to - unit);
-            for (int i = lane; i < n + lane; i += WARPS) {
-                if (lane < WARPS && i < n && !lost) {
-                    const int token = (place.tile + i) * kUnit, row = token & page_mask, slot = lane * L::kStages + count % L::kStages;
-                    const int page0 = page_of(a, place.seq, token, place.s.len), page1 = whole_units ? -1 : page_of(a, place.seq, token + 16, place.s.len);
-                    if (count >= L::kStages) lost = !umma::mbar_wait(base + L::kEmpty + 8 * slot, (count / L::kStages - 1) & 1);
-                    const uint32_t full = base + L::kFull + 8 * slot, to_codes = base + slot * S::kStage, to_heads = base + L::kHeads + slot * S::kHeadStage;
-                    const int run = whole_units ? kUnit : 16;  // tokens of a copy
-                    const int there = whole_units ? (page0 >= 0 ? 3 : 0) : (page0 >= 0 ? 1 : 0) + (page1 >= 0 ? 2 : 0);
-                    if (!lost) {
-                        *reinterpret_cast<int*>(smem + L::kThere + 4 * slot) = there;
-                        umma::mbar_arrive_expect_tx(full, __popc(there) * 16 * (2 * S::kRowBytes + 2 * S::kHeads * 4));
+    // ---- fetching: the units of a segment's part, every WARPS-th for this warp.  Lane j knows where the rows of the j-th unit ahead are: the first and
+    // the last 16 tokens' keys, as bytes from the pages' begin, negative where the cache has no such page.
+    const int page_log2 = a.pages.page_log2, page_mask = (1 << page_log2) - 1;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * L::kStages * S::kStage;
+    const uint8_t* codes = reinterpret_cast<const uint8_t*>(a.pages.words) + lane * 16;
+    const uint32_t value_bytes = (uint32_t)S::kRowBytes << page_log2;
+    const uint32_t to_chunk = ring + S::place(lane / S::kChunks, lane % S::kChunks * 16);
+    const uint32_t to_odd_chunk = ring + S::place(lane / S::kChunks + 4, lane % S::kChunks * 16) - 4 * S::kRowBytes;  // four rows of 256 values further
+    const uint32_t to_head = ring + S::kHeadsAt + ((lane / 16) * kUnit + lane % 16) * S::kHeads * 4;
+    const int64_t from_head = ((int64_t)(2 * S::kRowBytes + (lane / 16) * S::kHeads * 4) << page_log2) + lane % 16 * S::kHeads * 4 - lane * 16;  // from a page's first key
+    int64_t keys_of[2];
+    uint32_t there = 0;  // bits 2 s and 2 s + 1: the tokens of the unit in stage s have a page
+    int stage = 0;
+    const auto look_up = [&](int k0, int n) {  // from the warp's unit k0 on
+        const int i = warp + (k0 + lane) * WARPS;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int page = h == 0 ? page0 : page1, row0 = h == 0 ? row : 0;  // pages of 16 tokens begin with the half
-                            if (page < 0) continue;
-                            const uint32_t rec = (uint32_t)page * (uint32_t)a.pages.n_heads + (uint32_t)place.head;
-                            load_lines(to_codes + h * half_step, &map, row0 * S::kRowBytes / 128, rec, full);
-                            load_lines(to_codes + S::kPlane + h * half_step, &map, (page_size + row0) * S::kRowBytes / 128, rec, full);
-                            const uint8_t* heads = pages + (uint64_t)rec * record_bytes + (((uint32_t)(2 * S::kRowBytes) << a.pages.page_log2) + row0 * S::kHeads * 4);
-                            load_bytes(to_heads + h * 16 * S::kHeads * 4, heads, run * S::kHeads * 4, full);
-                            load_bytes(to_heads + (kUnit + h * 16) * S::kHeads * 4, heads + (S::kHeads * 4 << a.pages.page_log2), run * S::kHeads * 4, full);
-                        }
-                    }
-                    ++count;
-                }
-                __syncwarp();
-            }
-            unit += n;
-            next_segment<kRows>(a, place);
+        for (int h = 0; h < 2; ++h) {
+            const int token = (place.tile + i) * kUnit + 16 * h, page = i < n ? page_of(a, place.seq, token, place.s.len) : -1;
+            keys_of[h] = page < 0 ? -1 : (((int64_t)page * a.pages.n_heads + place.head) * (row_words(DIM) * 4) << page_log2) + (token & page_mask) * S::kRowBytes;
         }
-        return;
-    }
+    };
+    // Fetches the warp's unit k into the stage `to`; its group of copies is empty where there is none.
+    const auto fetch = [&](int k, int units, int to) {
+        if (k < units) {
+            uint32_t got = 0;
+            const int row = (place.tile + warp + k * WARPS) * kUnit;
+            const uint32_t stage_at = to * S::kStage;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int64_t at = __shfl_sync(0xFFFFFFFFu, keys_of[h], k & 31);
+                if (at < 0) continue;
+                got |= 1u << h;
+                const uint8_t* key = codes + at;
+                const uint8_t* value = key + value_bytes;
+                const uint8_t* head = key + (from_head - ((row + 16 * h) & page_mask) * (S::kRowBytes - S::kHeads * 4));
+#pragma unroll
+                for (int i = 0; i < S::kRowBytes / 32; ++i) {  // 32 chunks at a time
+                    const uint32_t to_at = (DIM == 256 && (i & 1) ? to_odd_chunk : to_chunk) + stage_at + (16 * h * S::kRowBytes + i * 512);
+                    copy16(to_at, key + i * 512);
+                    copy16(to_at + S::kPlane, value + i * 512);
+                }
+#pragma unroll
+                for (int i = 0; i < S::kHeads; ++i) copy4(to_head + stage_at + (16 * h * S::kHeads + i) * 4, head + 4 * i);
+            }
+            there = (there & ~(3u << 2 * to)) | got << 2 * to;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // The first units of a segment's part; returns how many the warp has.
+    const auto begin = [&](int n) {
+        const int units = n > warp ? (n - warp - 1) / WARPS + 1 : 0;
+        look_up(0, n);
+#pragma unroll 1
+        for (int k = 0; k < L::kStages - 1; ++k) fetch(k, units, (stage + k) % L::kStages);
+        return units;
+    };
+    int n = min(place.tiles - place.tile, to - from), my_units = begin(n);
     // where a lane reads in a stage: keys of token g, values of tokens 2 t and 2 t + 1, and their heads
-    const int key_at = S::place(S::placed(g), t * (DIM / 8)), key_at_1 = S::place(S::placed(g), t * (DIM / 8) + 16);  // of 256 values, the second half
-    const int value_at = S::kPlane + S::place(S::placed(2 * t), g * (DIM / 16)), value_at_1 = S::kPlane + S::place(S::placed(2 * t + 1), g * (DIM / 16));
-    const int head_at = S::placed(g) * S::kHeads * 4;
-    const int pair_at = (kUnit + S::placed(2 * t)) * S::kHeads * 4 + (DIM == 256 ? g / 4 * 4 : 0), pair_at_1 = (kUnit + S::placed(2 * t + 1)) * S::kHeads * 4 + (DIM == 256 ? g / 4 * 4 : 0);
-    int stage = 0, phase = 0;
-    bool lost = false;  // a wait gave up: results are not numbers
+    const int key_at = S::place(placed(g), t * (DIM / 8)), key_at_1 = S::place(placed(g), t * (DIM / 8) + 16);  // of 256 values, the second half
+    const int value_at = S::kPlane + S::place(placed(2 * t), g * (DIM / 16)), value_at_1 = S::kPlane + S::place(placed(2 * t + 1), g * (DIM / 16));
+    const int head_at = S::kHeadsAt + placed(g) * S::kHeads * 4;
+    const int pair_at = S::kHeadsAt + (kUnit + placed(2 * t)) * S::kHeads * 4 + (DIM == 256 ? g / 4 * 4 : 0);
+    const int pair_at_1 = S::kHeadsAt + (kUnit + placed(2 * t + 1)) * S::kHeads * 4 + (DIM == 256 ? g / 4 * 4 : 0);
+    const Exponents exponents;
 
     // ---- one (sequence, head, tile of queries) after the other
     for (int unit = from; unit < to;) {
-        const int n = min(place.tiles - place.tile, to - unit);
         raw.put(a, queries);
-        sync_workers<kThreads>();
+        __syncthreads();
         float o[NB][S::kTiles][4], bits[NB][S::kBitTiles][4], m[NB][2], l[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -436,16 +437,15 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
             l[nb][0] = l[nb][1] = 0.0f;
         }
         const int drafted = place.s.len - place.s.count;
-        for (int i = warp; i < n; i += WARPS) {
-            const int slot = warp * L::kStages + stage;
-            if (lost || !umma::mbar_wait_warp(base + L::kFull + 8 * slot, phase)) {
-                lost = true;
-                break;
-            }
-            const uint8_t *at = smem + slot * S::kStage, *heads = smem + L::kHeads + slot * S::kHeadStage;
-            const int there = *reinterpret_cast<const int*>(smem + L::kThere + 4 * slot);
-            const auto head_word = [&](int byte) { return *reinterpret_cast<const uint32_t*>(heads + byte); };
-            const int token0 = (place.tile + i) * kUnit;
+        for (int k = 0; k < my_units; ++k) {
+            __syncwarp();  // every lane has read the stage that is filled next
+            if ((k + L::kStages - 1) % 32 == 0) look_up(k + L::kStages - 1, n);
+            fetch(k + L::kStages - 1, my_units, stage == 0 ? L::kStages - 1 : stage - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 1) : "memory");
+            __syncwarp();
+            const uint8_t* at = smem + (warp * L::kStages + stage) * S::kStage;
+            const auto head_word = [&](int byte) { return *reinterpret_cast<const uint32_t*>(at + byte); };
+            const int token0 = (place.tile + warp + k * WARPS) * kUnit;
 
             // scores: [group of 16 tokens][tile of 8 queries][token g: query 2 t, 2 t + 1; token g + 8: the same]
             float s[2][NB][4], step[2][2];
@@ -463,11 +463,10 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
                 uint32_t kw[2][S::kKeyWords], kh[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    // eight rows of 64 (128, 256) values are 256 (512, 1024) bytes, and the swizzle turns with every 1024
-                    const int rows = h * half_step + 8 * e * S::kRowBytes, turn = DIM == 64 ? (h * (half_step >> 3 & 0x40) + 0x20 * e) : DIM == 128 ? 0x40 * e : 0;
-                    if (DIM == 64) load_words<2>(at + ((key_at ^ turn) + rows), kw[e]);
-                    else load_words<4>(at + ((key_at ^ turn) + rows), kw[e]);
-                    if (DIM == 256) load_words<4>(at + (key_at_1 + rows), kw[e] + S::kKeyWords / 2);
+                    const int rows = (16 * h + 8 * e) * S::kRowBytes;
+                    if (DIM == 64) load_words<2>(at + key_at + rows, kw[e]);
+                    else load_words<4>(at + key_at + rows, kw[e]);
+                    if (DIM == 256) load_words<4>(at + key_at_1 + rows, kw[e] + S::kKeyWords / 2);
                     kh[e] = head_word(head_at + (16 * h + 8 * e) * S::kHeads * 4 + (DIM == 256 ? t / 2 * 4 : 0));
                     step[h][e] = __uint_as_float(kh[e] & 0xFFFF0000u);
                 }
@@ -523,8 +522,8 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
                             for (int h = 0; h < 2; ++h)
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
-                                    const int token = token0 + 16 * h + 8 * e + S::placed(g), j = token - drafted;
-                                    const bool yes = token < place.s.len && (there >> h & 1) &&
+                                    const int token = token0 + 16 * h + 8 * e + placed(g), j = token - drafted;
+                                    const bool yes = token < place.s.len && (there >> (2 * stage + h) & 1) &&
                                                      (j < 0 || (a.tree ? j < 64 && (who >> j & 1) : j <= (int)who));
                                     seen[nb] |= (uint32_t)yes << (4 * h + 2 * e + c);
                                 }
@@ -595,7 +594,7 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
                             if (kWeights == 2) p[h][nb][e][kWeights - 1] = transposed(rest_pair(w[0], w[1], pair));
                         }
             };
-            if (token0 + kUnit <= drafted && there == 3) softmax(std::true_type());
+            if (token0 + kUnit <= drafted && (there >> 2 * stage & 3) == 3) softmax(std::true_type());
             else softmax(std::false_type());
 
             // values
@@ -604,9 +603,9 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
                 uint32_t vw[4][S::kValueWords], vh[4];  // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int e = k >> 1, rows = h * half_step + 8 * e * S::kRowBytes, turn = DIM == 64 ? (h * (half_step >> 3 & 0x40) + 0x20 * e) : DIM == 128 ? 0x40 * e : 0;
-                    load_words<S::kValueWords>(at + (((k & 1 ? value_at_1 : value_at) ^ turn) + rows), vw[k]);
-                    vh[k] = head_word((k & 1 ? pair_at_1 : pair_at) + (16 * h + 8 * e) * S::kHeads * 4);
+                    const int rows = 16 * h + 8 * (k >> 1);
+                    load_words<S::kValueWords>(at + (k & 1 ? value_at_1 : value_at) + rows * S::kRowBytes, vw[k]);
+                    vh[k] = head_word((k & 1 ? pair_at_1 : pair_at) + rows * S::kHeads * 4);
                 }
                 const auto add = [&](float (&acc)[NB][S::kTiles][4], int tile, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
@@ -619,8 +618,8 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
 #pragma unroll
                     for (int high = 0; high < 2; ++high) {
                         const uint32_t x = __byte_perm(vw[0][w], vw[1][w], high ? 0x7632 : 0x5410), y = __byte_perm(vw[2][w], vw[3][w], high ? 0x7632 : 0x5410);
-                        add(o, 4 * w + 2 * high, even_values(x), odd_values(x), even_values(y), odd_values(y));
-                        add(o, 4 * w + 2 * high + 1, even_values(x >> 8), odd_values(x >> 8), even_values(y >> 8), odd_values(y >> 8));
+                        add(o, 4 * w + 2 * high, exponents.even_values(x), exponents.odd_values(x), exponents.even_values(y), exponents.odd_values(y));
+                        add(o, 4 * w + 2 * high + 1, exponents.even_values(x >> 8), exponents.odd_values(x >> 8), exponents.even_values(y >> 8), exponents.odd_values(y >> 8));
                     }
                 const int shift = DIM == 64 ? g : DIM == 128 ? 2 * g : 4 * (g & 3);
                 const uint32_t x = __byte_perm(vh[0], vh[1], 0x5410) >> shift << 10, y = __byte_perm(vh[2], vh[3], 0x5410) >> shift << 10;
@@ -633,16 +632,7 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
                             mma(bits[nb][k], x & (0x04000400u << (2 * k)), x & (0x08000800u << (2 * k)), y & (0x04000400u << (2 * k)), y & (0x08000800u << (2 * k)),
                                 p[h][nb][0][part], p[h][nb][1][part]);
             }
-            __syncwarp();  // every lane has read
-            if (lane == 0) umma::mbar_arrive(base + L::kEmpty + 8 * slot);
-            if (++stage == L::kStages) {
-                stage = 0;
-                phase ^= 1;
-            }
-        }
-        if (lost) {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = __uint_as_float(0x7FC00000u);
+            if (++stage == L::kStages) stage = 0;
         }
 
         // ---- the warps' parts into one
@@ -660,10 +650,15 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
                     joining.l[8 * nb + 2 * t + c][warp] = x;
                 }
             }
-        Place next = place;
-        next_segment<kRows>(a, next);
-        if (unit + n < to) raw.load(a, next);  // the next tile's queries, on their way meanwhile
-        sync_workers<kThreads>();
+        const Place done = place;
+        const int done_units = n;
+        next_segment<kRows>(a, place);
+        if (unit + done_units < to) {  // the next tile's queries and first units, on their way meanwhile
+            raw.load(a, place);
+            n = min(place.tiles, to - unit - done_units);
+            my_units = begin(n);
+        }
+        __syncthreads();
         // of row r: the largest maximum of the warps
         const auto top_of = [&](int r) {
             float top = -INFINITY;
@@ -674,8 +669,8 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
         const int q_heads = a.group * a.pages.n_heads;
         // row r of the tile: where its result goes
         const auto row_of = [&](int r) {
-            const int row = place.qtile * kRows + r;
-            return (int64_t)(place.s.first + row / a.group) * q_heads + place.head * a.group + row % a.group;
+            const int row = done.qtile * kRows + r;
+            return (int64_t)(done.s.first + row / a.group) * q_heads + done.head * a.group + row % a.group;
         };
         const auto put = [&](int r, int d, float x, float y) {
             if (PARTS == 2) *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + row_of(r) * DIM + d) = __floats2bfloat162_rn(x, y);
@@ -686,10 +681,10 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
         };
         // a CTA's parts: of the segment that began before it, and of the one that goes on behind it
         constexpr int kPart = kRows * (DIM + 2);
-        float* partial = a.partials + ((int64_t)blockIdx.x * 2 + (place.tile > 0 ? 0 : 1)) * kPart;
+        float* partial = a.partials + ((int64_t)blockIdx.x * 2 + (done.tile > 0 ? 0 : 1)) * kPart;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            if (nb > 0) sync_workers<kThreads>();  // the tile before is read
+            if (nb > 0) __syncthreads();  // the tile before is read
             if (warp < live) {
                 float scale[2];
 #pragma unroll
@@ -706,7 +701,7 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
                     }
                 }
             }
-            sync_workers<kThreads>();
+            __syncthreads();
             for (int at = threadIdx.x; at < 8 * DIM / 2; at += kThreads) {
                 const int r = 8 * nb + at / (DIM / 2), d = at % (DIM / 2) * 2;
                 if (r >= rows) continue;
@@ -735,15 +730,15 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
             }
         }
         // ---- the CTAs' parts into one: those from the CTA with the segment's first unit to the one with its last
-        sync_workers<kThreads>();  // joined, and the parts written
+        __syncthreads();  // joined, and the parts written
         if (!whole) {
-            const int first_cta = cut.cta_of(unit - place.tile), parts = cut.cta_of(unit - place.tile + place.tiles - 1) - first_cta + 1;
+            const int first_cta = cut.cta_of(unit - done.tile), parts = cut.cta_of(unit - done.tile + done.tiles - 1) - first_cta + 1;
             if (threadIdx.x == 0) {
                 uint32_t arrived;
                 asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(arrived) : "l"(a.counters + first_cta) : "memory");
                 is_last = arrived == (uint32_t)(parts - 1);
             }
-            sync_workers<kThreads>();
+            __syncthreads();
             if (is_last) {
                 constexpr int kAtOnce = 10;
                 for (int at = threadIdx.x; at < rows * (DIM / 4); at += kThreads) {
@@ -787,27 +782,13 @@ k_cache_attend(const __grid_constant__ Attend a, const __grid_constant__ CUtenso
                 if (threadIdx.x == 0) a.counters[first_cta] = 0;
             }
         }
-        unit += n;
-        place = next;
+        unit += done_units;
     }
-    if (lost) {  // what was on its way when the wait gave up has to land before the memory is another's
-        for (int i = 0; i < L::kStages; ++i) umma::mbar_wait_warp(base + L::kFull + 8 * (warp * L::kStages + i), phase);
-    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 constexpr int kMostRows = 16;
 int64_t scratch_bytes_of(int head_dim) { return 4 * kMostCtas + (int64_t)kMostCtas * 2 * kMostRows * (head_dim + 2) * 4; }
-
-// The codes of all records as lines of 128 bytes, [n_records][keys and values]
-template <int DIM>
-int make_map(const Attend& a, CUtensorMap* map) {
-    memset(map, 0, sizeof(*map));
-    if (a.pages.n_pages == 0) return 0;  // nothing is fetched
-    const uint64_t page = 1ull << a.pages.page_log2, record_bytes = page * row_words(DIM) * 4;
-    const cuuint64_t dims[3] = {128, 2 * page * Shape<DIM>::kRowBytes / 128, (cuuint64_t)a.pages.n_pages * a.pages.n_heads}, strides[2] = {128, record_bytes};
-    const cuuint32_t box[3] = {128, (cuuint32_t)(Shape<DIM>::kLines * (a.pages.page_log2 > 4 ? 2 : 1)), 1}, step[3] = {1, 1, 1};
-    return umma::encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.pages.words, dims, strides, box, step);
-}
 
 template <int DIM, int PARTS, int NB, int WARPS>
 int launch_as(const Attend& a, cudaStream_t st) {
@@ -815,18 +796,16 @@ int launch_as(const Attend& a, cudaStream_t st) {
     static_assert(L::kBytes <= 227 * 1024, "shared memory");
     static_assert(8 * NB <= kMostRows, "scratch memory");
     const auto kernel = k_cache_attend<DIM, PARTS, NB, WARPS>;
-    CUtensorMap map;
-    if (int e = make_map<DIM>(a, &map)) return e;
     if (int e = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes), "cudaFuncSetAttribute")) return e;
     const int sms = sm_count(), grid = sms < kMostCtas ? sms : kMostCtas;
-    return launch_dependent("e8_cache_attention", kernel, (unsigned)grid, 32 * WARPS + 32, L::kBytes, st, a, map);
+    return launch_dependent("e8_cache_attention", kernel, (unsigned)grid, 32 * WARPS, L::kBytes, st, a);
 }
 
 template <int DIM, int PARTS>
 int launch(const Attend& a, cudaStream_t st) {
     const int64_t rows = ((int64_t)a.n_queries + a.n_seqs - 1) / a.n_seqs * a.group;  // of a cache head, on average
-    if (rows <= 8) return launch_as<DIM, PARTS, 1, DIM == 256 ? 7 : 11>(a, st);
-    return launch_as<DIM, PARTS, 2, 7>(a, st);
+    if (rows <= 8) return launch_as<DIM, PARTS, 1, 8>(a, st);
+    return launch_as<DIM, PARTS, 2, DIM == 256 && PARTS == 3 ? 6 : 8>(a, st);
 }
 
 }  // namespace

@@ -198,10 +198,10 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
 
-// Tensor map with the 128-byte swizzle and zero fill outside the tensor.  The driver entry point is looked up through the runtime so
+// Tensor map of a row-major bf16 matrix x[T, K] (row stride ldx): boxes of 64 (K) x box_rows, 128-byte
+// swizzle, zero fill outside the tensor.  The driver entry point is looked up through the runtime so
 // that the library does not link against the driver library.
-inline int encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* x, const cuuint64_t* dims, const cuuint64_t* strides,
-                      const cuuint32_t* box, const cuuint32_t* elem) {
+inline int make_bf16_map(CUtensorMap* map, const void* x, int K, int T, int64_t ldx, int box_rows = BM) {
     typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                     const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                     CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -213,8 +213,12 @@ inline int encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, cons
         if (qres != cudaDriverEntryPointSuccess || !fn) return fail(COSET_E_STATE, "cuTensorMapEncodeTiled is not available in this driver");
         encode = (EncodeTiled)fn;
     }
+    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)T};
+    const cuuint64_t strides[1] = {(cuuint64_t)ldx * 2};  // bytes between rows; a multiple of 16 (ldx % 8 == 0)
+    const cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
+    const cuuint32_t elem[2] = {1, 1};
     const auto make = [&]() {
-        return encode(map, type, rank, const_cast<void*>(x), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+        return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                       CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     };
     CUresult r = make();
@@ -226,15 +230,6 @@ inline int encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, cons
     }
     if (r != CUDA_SUCCESS) return fail(COSET_E_BADARG, "cuTensorMapEncodeTiled failed with code %d", (int)r);
     return 0;
-}
-
-// Tensor map of a row-major bf16 matrix x[T, K] (row stride ldx): boxes of 64 (K) x box_rows.
-inline int make_bf16_map(CUtensorMap* map, const void* x, int K, int T, int64_t ldx, int box_rows = BM) {
-    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)T};
-    const cuuint64_t strides[1] = {(cuuint64_t)ldx * 2};  // bytes between rows; a multiple of 16 (ldx % 8 == 0)
-    const cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
-    const cuuint32_t elem[2] = {1, 1};
-    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, dims, strides, box, elem);
 }
 
 }  // namespace umma
