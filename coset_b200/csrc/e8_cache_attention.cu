@@ -34,9 +34,12 @@ namespace {
 constexpr int kUnit = 32;         // tokens of a warp's step
 constexpr int kLeastUnits = 4;    // of a CTA
 constexpr int kLeastSize = -90;   // exponent of a value's step as far as the running maximum goes: sums of p / 2^kLeastSize stay finite
-constexpr int kMostCtas = 152;    // counters in the scratch memory
+constexpr int kMostCtas = 304;    // counters in the scratch memory
 constexpr int kExact = 0x4B400000;  // the bits of kExactly = 1.5 2^23; a whole number of up to 22 bits added to them is added to it
 constexpr float kExactly = 12582912.0f;
+constexpr float kNothing = -3.402823466e38f;  // running maximum of a row that has seen nothing
+// What a segment costs a CTA beyond its units, in units: its queries, its first loads' latency, its joining.  The cut counts it.
+constexpr int kSegment = 16;
 
 // The row of a group of 8 that stands in row r of an operand: 0 1 2 3 5 4 7 6.  With the swizzle below no read of codes has a bank conflict.
 __device__ __forceinline__ int placed(int r) { return r ^ ((r >> 2) & 1); }
@@ -142,7 +145,7 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
 // A tile of queries of one head in shared memory, in the order of the operands.  Part 0 of a number is its top byte, with the sign.
 template <int DIM, int PARTS, int NB>
 struct Queries {
-    uint2 words[NB][PARTS][DIM / 32][32];                 // of word w: values 0, 2, 4, 6 and 1, 3, 5, 7 of its block
+    uint2 words[NB][DIM / 32][32][PARTS];                 // of word w: values 0, 2, 4, 6 and 1, 3, 5, 7 of its block
     uint2 blocks[NB][PARTS][Shape<DIM>::kBitTiles][32];   // half the sums of four blocks: the part's bytes, and 64ths of what the top part is too small for
     int start[PARTS][8 * NB];                             // kExact - 8 sum of the part
     float factor[8 * NB];                                 // from a sum to a score in powers of two, but for the key's step
@@ -152,8 +155,9 @@ struct Queries {
 template <int DIM, int NB, int WARPS>
 struct Joining {
     static constexpr int kStride = DIM * 18 / 16 + 4;  // rows of 16 values lie 18 apart: no bank conflicts between lanes
-    float o[WARPS][8][kStride];
-    float m[8 * NB][16], l[8 * NB][16];  // of the warps
+    float o[WARPS][8 * NB][kStride];      // the warps' sums of w f,
+    float bits[WARPS][8 * NB][DIM / 8];   // of w c by block,
+    float m[8 * NB][WARPS], l[8 * NB][WARPS];  // their maxima and sums of p
     static __device__ __forceinline__ int at(int d) { return d + 2 * (d / 16); }
 };
 
@@ -162,14 +166,18 @@ struct Place {
     Sequence s;
     int seq, head, qtile, qtiles, tile, tiles;
 };
+// A segment that other CTAs have parts of, to be joined by the last of them
+struct Pending {
+    Place place;
+    int first_cta, parts, slot, is_last;
+};
 template <int DIM, int PARTS, int NB, int WARPS>
 struct Layout {
-    static constexpr int kStages = WARPS > 12 || DIM == 256 ? 2 : 3;
+    static constexpr int kStages = DIM == 256 ? 2 : 3;
     static constexpr int kQueries = WARPS * kStages * Shape<DIM>::kStage;
-    static constexpr int kJoining = kQueries + (int)sizeof(Queries<DIM, PARTS, NB>);
-    static constexpr int kLast = kJoining + (int)sizeof(Joining<DIM, NB, WARPS>);
-    static constexpr int kBytes = kLast + 16;
-    static_assert(WARPS <= 16, "rows of Joining::m");
+    static constexpr int kJoining = kQueries + 2 * (int)sizeof(Queries<DIM, PARTS, NB>);
+    static constexpr int kPending = kJoining + (int)sizeof(Joining<DIM, NB, WARPS>);
+    static constexpr int kBytes = kPending + 2 * (int)sizeof(Pending);
 };
 
 template <int ROWS>
@@ -191,13 +199,13 @@ __device__ __forceinline__ void next_segment(const Attend& a, Place& p) {
     } while (p.qtiles == 0);
 }
 
-// The units' cut: CTA c has base units, and one more where c < more.
+// The cut of all segments, each as long as its units and kSegment: CTA c has base of that, and one more where c < more.
 struct Cut {
     int base, more;
     __device__ __forceinline__ int from(int cta) const { return base * cta + min(cta, more); }
-    __device__ __forceinline__ int cta_of(int unit) const {
+    __device__ __forceinline__ int cta_of(int at) const {
         const int longer = more * (base + 1);
-        return unit < longer ? unit / (base + 1) : more + (unit - longer) / base;
+        return at < longer ? at / (base + 1) : more + (at - longer) / base;
     }
 };
 
@@ -258,7 +266,7 @@ struct QueryBlocks {
             const uint32_t pick = byte * 0x11 + 0x40;
             const uint32_t even = __byte_perm(__byte_perm(q[0], q[2], pick), __byte_perm(q[4], q[6], pick), 0x5410);
             const uint32_t odd = __byte_perm(__byte_perm(q[1], q[3], pick), __byte_perm(q[5], q[7], pick), 0x5410);
-            s.words[r / 8][j][word][lane] = make_uint2(even, odd);
+            s.words[r / 8][word][lane][j] = make_uint2(even, odd);
             part_sum[j] = j == 0 ? __dp4a((int)even, 0x01010101, __dp4a((int)odd, 0x01010101, 0)) : (int)__dp4a(even, 0x01010101u, __dp4a(odd, 0x01010101u, 0u));
             sum = sum * 256 + part_sum[j];
         }
@@ -289,17 +297,36 @@ struct QueryBlocks {
     }
 };
 
-template <int DIM, int PARTS, int NB, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, 1)
+// Half a block's bit, from the sum over what the bit stands for as a 16-bit number
+template <int DIM>
+__device__ __forceinline__ float half_of_bit(int block) { return 0.5f / of_bit(block % (DIM / 64)); }
+// Row r of a tile of `rows` queries: where its result goes
+__device__ __forceinline__ int64_t result_row(const Attend& a, const Place& p, int rows, int r) {
+    const int row = p.qtile * rows + r, query = row / a.group;
+    return (int64_t)(p.s.first + query) * (a.group * a.pages.n_heads) + p.head * a.group + row - query * a.group;
+}
+template <int PARTS, int DIM>
+__device__ __forceinline__ void put_pair(const Attend& a, const Place& p, int rows, int r, int d, float x, float y) {
+    const int64_t at = result_row(a, p, rows, r) * DIM + d;
+    if (PARTS == 2) *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + at) = __floats2bfloat162_rn(x, y);
+    else *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(x, y);
+}
+__device__ __forceinline__ void put_lse(const Attend& a, const Place& p, int rows, int r, float highest, float sum) {
+    if (a.lse) a.lse[result_row(a, p, rows, r)] = highest == kNothing ? -INFINITY : (highest + log2f(sum)) * 0.69314718f;
+}
+
+template <int DIM, int PARTS, int NB, int WARPS, int CTAS>
+__global__ void __launch_bounds__(32 * WARPS, CTAS)
 k_cache_attend(const __grid_constant__ Attend a) {
     using S = Shape<DIM>;
     using L = Layout<DIM, PARTS, NB, WARPS>;
     constexpr int kRows = 8 * NB, kThreads = 32 * WARPS, kWeights = PARTS - 1;  // 16-bit parts of a weight
+    constexpr int kPart = kRows * (DIM + 2);  // floats of a CTA's part: maxima, sums, rows; it has one for a segment that began before it and one for one that goes on behind it
     constexpr float kSlack = PARTS == 3 ? 2.0f : 8.0f, kShift = PARTS == 3 ? 12.0f : 6.0f;  // weights reach 2^(1 + kSlack + kShift)
     extern __shared__ __align__(128) uint8_t smem[];
-    auto& queries = *reinterpret_cast<Queries<DIM, PARTS, NB>*>(smem + L::kQueries);
+    auto* const all_queries = reinterpret_cast<Queries<DIM, PARTS, NB>*>(smem + L::kQueries);
     auto& joining = *reinterpret_cast<Joining<DIM, NB, WARPS>*>(smem + L::kJoining);
-    int& is_last = *reinterpret_cast<int*>(smem + L::kLast);
+    auto* const pending = reinterpret_cast<Pending*>(smem + L::kPending);
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     grid_wait();
     grid_trigger();
@@ -311,7 +338,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
         if (b >= a.n_seqs) return (int64_t)0;
         place.seq = b;
         enter<kRows>(a, place);
-        return (int64_t)place.qtiles * a.pages.n_heads * place.tiles;
+        return (int64_t)place.qtiles * a.pages.n_heads * (place.tiles + kSegment);
     };
     const auto inclusive = [&](int64_t v) {
 #pragma unroll
@@ -326,7 +353,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
     int64_t units = units_of(lane), upto = inclusive(units);
     all += __shfl_sync(0xFFFFFFFFu, upto, 31);
     if (all < 1 || all > INT32_MAX) return;  // so many only from starts that overlap: the host refuses as much work
-    const int total = (int)all, ctas = min((int)gridDim.x, (total - 1) / kLeastUnits + 1);
+    const int total = (int)all, ctas = min((int)gridDim.x, (total - 1) / (kLeastUnits + kSegment) + 1);
     if (blockIdx.x >= ctas) return;
     const Cut cut = {total / ctas, total % ctas};
     const int from = cut.from(blockIdx.x), to = cut.from(blockIdx.x + 1);
@@ -340,8 +367,8 @@ k_cache_attend(const __grid_constant__ Attend a) {
             place.qtiles = __shfl_sync(0xFFFFFFFFu, place.qtiles, src);
             place.tiles = __shfl_sync(0xFFFFFFFFu, place.tiles, src);
             place.seq = b + src;
-            const int segment = rest / place.tiles;
-            place.tile = rest - segment * place.tiles;
+            const int segment = rest / (place.tiles + kSegment);
+            place.tile = rest - segment * (place.tiles + kSegment);
             place.head = segment / place.qtiles;
             place.qtile = segment - place.head * place.qtiles;
             break;
@@ -350,6 +377,12 @@ k_cache_attend(const __grid_constant__ Attend a) {
         const int64_t before = __shfl_sync(0xFFFFFFFFu, upto, 31);
         units = units_of(b + lane);
         upto = before + inclusive(units);
+    }
+    int at_unit = from;  // place in the cut
+    if (place.tile >= place.tiles) {  // behind the segment's last unit: on to the next one
+        at_unit += place.tiles + kSegment - place.tile;
+        if (at_unit >= to) return;
+        next_segment<kRows>(a, place);
     }
     QueryBlocks<DIM, PARTS, NB, WARPS> raw;
     raw.load(a, place);
@@ -410,7 +443,10 @@ k_cache_attend(const __grid_constant__ Attend a) {
         for (int k = 0; k < L::kStages - 1; ++k) fetch(k, units, (stage + k) % L::kStages);
         return units;
     };
-    int n = min(place.tiles - place.tile, to - from), my_units = begin(n);
+    int n = min(place.tiles - place.tile, to - at_unit), my_units = begin(n), buffer = 0, n_pending = 0;
+    uint32_t arrived[2] = {0, 0};  // of thread 0
+    raw.put(a, all_queries[0]);
+    __syncthreads();
     // where a lane reads in a stage: keys of token g, values of tokens 2 t and 2 t + 1, and their heads
     const int key_at = S::place(placed(g), t * (DIM / 8)), key_at_1 = S::place(placed(g), t * (DIM / 8) + 16);  // of 256 values, the second half
     const int value_at = S::kPlane + S::place(placed(2 * t), g * (DIM / 16)), value_at_1 = S::kPlane + S::place(placed(2 * t + 1), g * (DIM / 16));
@@ -420,9 +456,8 @@ k_cache_attend(const __grid_constant__ Attend a) {
     const Exponents exponents;
 
     // ---- one (sequence, head, tile of queries) after the other
-    for (int unit = from; unit < to;) {
-        raw.put(a, queries);
-        __syncthreads();
+    while (true) {
+        const auto& queries = all_queries[buffer];
         float o[NB][S::kTiles][4], bits[NB][S::kBitTiles][4], m[NB][2], l[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -433,7 +468,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
 #pragma unroll
                 for (int k = 0; k < S::kBitTiles; ++k) bits[nb][k][i] = 0.0f;
             }
-            m[nb][0] = m[nb][1] = -INFINITY;
+            m[nb][0] = m[nb][1] = kNothing;
             l[nb][0] = l[nb][1] = 0.0f;
         }
         const int drafted = place.s.len - place.s.count;
@@ -474,13 +509,18 @@ k_cache_attend(const __grid_constant__ Attend a) {
                 for (int w = 0; w < S::kKeyWords; ++w) {
                     const uint32_t x0 = kw[0][w] & 0x0F0F0F0Fu, x1 = kw[1][w] & 0x0F0F0F0Fu, x2 = kw[0][w] >> 4 & 0x0F0F0F0Fu, x3 = kw[1][w] >> 4 & 0x0F0F0F0Fu;
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const auto& q = queries.words[nb][w][lane];
+                        if (PARTS == 2) {
+                            const uint4 both = *reinterpret_cast<const uint4*>(&q[0]);
+                            mma_bytes<true>(sum[0][nb], x0, x1, x2, x3, both.x, both.y);
+                            mma_bytes<false>(sum[1][nb], x0, x1, x2, x3, both.z, both.w);
+                        } else {
+                            mma_bytes<true>(sum[0][nb], x0, x1, x2, x3, q[0].x, q[0].y);
 #pragma unroll
-                        for (int j = 0; j < PARTS; ++j) {
-                            const uint2 q = queries.words[nb][j][w][lane];
-                            if (j == 0) mma_bytes<true>(sum[j][nb], x0, x1, x2, x3, q.x, q.y);
-                            else mma_bytes<false>(sum[j][nb], x0, x1, x2, x3, q.x, q.y);
+                            for (int j = 1; j < PARTS; ++j) mma_bytes<false>(sum[j][nb], x0, x1, x2, x3, q[j].x, q[j].y);
                         }
+                    }
                 }
 #pragma unroll
                 for (int k = 0; k < S::kBitTiles; ++k) {
@@ -502,100 +542,99 @@ k_cache_attend(const __grid_constant__ Attend a) {
                         float x = __int_as_float(sum[0][nb][i4]) - kExactly;
 #pragma unroll
                         for (int j = 1; j < PARTS; ++j) x = __fmaf_rn(x, 256.0f, __int_as_float(sum[j][nb][i4]) - kExactly);
-                        s[h][nb][i4] = x * step[h][i4 / 2];
+                        s[h][nb][i4] = x;
                     }
             }
 
             // softmax
-            uint32_t p[2][NB][2][kWeights];  // weights as 16-bit pairs of queries, [group][tile][token g, g + 8][part]
-            const auto softmax = [&](auto every) {
-                constexpr bool kAll = decltype(every)::value;
-                uint32_t seen[NB];  // bit 4 h + 2 e + c: token 16 h + 8 e + g is seen by query 2 t + c
-                if (!kAll) {
+            const bool all_seen = token0 + kUnit <= drafted && (there >> 2 * stage & 3) == 3;
+            float value_step[2][2], size[2][2], lag = -INFINITY, top[NB][2];
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        seen[nb] = 0;
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const uint64_t who = queries.bits[8 * nb + 2 * t + c];
-#pragma unroll
-                            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    const int token = token0 + 16 * h + 8 * e + placed(g), j = token - drafted;
-                                    const bool yes = token < place.s.len && (there >> (2 * stage + h) & 1) &&
-                                                     (j < 0 || (a.tree ? j < 64 && (who >> j & 1) : j <= (int)who));
-                                    seen[nb] |= (uint32_t)yes << (4 * h + 2 * e + c);
-                                }
-                        }
-                    }
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t v = head_word(head_at + (kUnit + 16 * h + 8 * e) * S::kHeads * 4);
+                    value_step[h][e] = __uint_as_float(v & 0xFFFF0000u);
+                    size[h][e] = fmaxf(__uint_as_float(0x4B400000u + (v >> 23 & 255u)) - (kExactly + 127.0f), (float)kLeastSize);
                 }
-                const auto sees = [&](int nb, int h, int e, int c) { return kAll || (seen[nb] >> (4 * h + 2 * e + c) & 1); };
-                float value_step[2][2], size[2][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const float2 factor = *reinterpret_cast<const float2*>(&queries.factor[8 * nb + 2 * t]);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const uint32_t v = head_word(head_at + (kUnit + 16 * h + 8 * e) * S::kHeads * 4);
-                        value_step[h][e] = __uint_as_float(v & 0xFFFF0000u);
-                        size[h][e] = fmaxf(__uint_as_float(0x4B400000u + (v >> 23 & 255u)) - (kExactly + 127.0f), (float)kLeastSize);
+                        s[h][nb][2 * e] *= step[h][e] * factor.x;
+                        s[h][nb][2 * e + 1] *= step[h][e] * factor.y;
                     }
-                float lag = -INFINITY, top[NB][2], f[NB][2];
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const float2 factor = *reinterpret_cast<const float2*>(&queries.factor[8 * nb + 2 * t]);
-                    f[nb][0] = factor.x;
-                    f[nb][1] = factor.y;
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        top[nb][c] = -INFINITY;
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                if (sees(nb, h, e, c)) top[nb][c] = larger(top[nb][c], __fmaf_rn(s[h][nb][2 * e + c], f[nb][c], size[h][e]));
-                        if (kAll || top[nb][c] != -INFINITY) lag = larger(lag, top[nb][c] - m[nb][c]);
-                    }
-                }
-                if (__any_sync(0xFFFFFFFFu, !(lag <= kSlack + kShift))) {
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float x = top[nb][c];
-#pragma unroll
-                            for (int d = 4; d < 32; d *= 2) x = larger(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
-                            x = larger(m[nb][c], x - kShift);
-                            const float keep = x == -INFINITY ? 1.0f : exp2_of(m[nb][c] - x);
-                            m[nb][c] = x;
-                            l[nb][c] *= keep;
-#pragma unroll
-                            for (int k = 0; k < S::kTiles; ++k) { o[nb][k][c] *= keep; o[nb][k][c + 2] *= keep; }
-#pragma unroll
-                            for (int k = 0; k < S::kBitTiles; ++k) { bits[nb][k][c] *= keep; bits[nb][k][c + 2] *= keep; }
-                        }
-                }
+            }
+            if (!all_seen) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int c = 0; c < 2; ++c) {
+                        const uint64_t who = queries.bits[8 * nb + 2 * t + c];
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float w[2];
+                        for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                float x = exp2_of(__fmaf_rn(s[h][nb][2 * e + c], f[nb][c], -m[nb][c]));
-                                w[c] = x * value_step[h][e];
-                                if (!sees(nb, h, e, c)) x = w[c] = 0.0f;
-                                l[nb][c] += x;
+                            for (int e = 0; e < 2; ++e) {
+                                const int token = token0 + 16 * h + 8 * e + placed(g), j = token - drafted;
+                                const bool seen = token < place.s.len && (there >> (2 * stage + h) & 1) && (j < 0 || (a.tree ? j < 64 && (who >> j & 1) : j <= (int)who));
+                                if (!seen) s[h][nb][2 * e + c] = -INFINITY;
                             }
-                            const uint32_t pair = half_pair(w[0], w[1]);
-                            p[h][nb][e][0] = transposed(pair);
-                            if (kWeights == 2) p[h][nb][e][kWeights - 1] = transposed(rest_pair(w[0], w[1], pair));
-                        }
-            };
-            if (token0 + kUnit <= drafted && (there >> 2 * stage & 3) == 3) softmax(std::true_type());
-            else softmax(std::false_type());
+                    }
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    top[nb][c] = s[0][nb][c] + size[0][0];
+                    top[nb][c] = larger(top[nb][c], s[0][nb][2 + c] + size[0][1]);
+                    top[nb][c] = larger(top[nb][c], s[1][nb][c] + size[1][0]);
+                    top[nb][c] = larger(top[nb][c], s[1][nb][2 + c] + size[1][1]);
+                    lag = larger(lag, top[nb][c] - m[nb][c]);
+                }
+            if (__any_sync(0xFFFFFFFFu, !(lag <= kSlack + kShift))) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float x = top[nb][c];
+#pragma unroll
+                        for (int d = 4; d < 32; d *= 2) x = larger(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
+                        x = larger(m[nb][c], x - kShift);
+                        const float keep = exp2_of(m[nb][c] - x);
+                        m[nb][c] = x;
+                        l[nb][c] *= keep;
+#pragma unroll
+                        for (int k = 0; k < S::kTiles; ++k) { o[nb][k][c] *= keep; o[nb][k][c + 2] *= keep; }
+#pragma unroll
+                        for (int k = 0; k < S::kBitTiles; ++k) { bits[nb][k][c] *= keep; bits[nb][k][c + 2] *= keep; }
+                    }
+            }
+            uint32_t p[2][NB][2][kWeights];  // weights as 16-bit pairs of queries, [group][tile][token g, g + 8][part]
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) {
+                        const float x = exp2_of(s[h][nb][i4] - m[nb][i4 & 1]);
+                        l[nb][i4 & 1] += x;
+                        s[h][nb][i4] = x * value_step[h][i4 >> 1];
+                        if (!all_seen && x == 0.0f) s[h][nb][i4] = 0.0f;  // whatever stands in a place that is not seen
+                    }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float w0 = s[h][nb][2 * e], w1 = s[h][nb][2 * e + 1];
+                        const uint32_t pair = half_pair(w0, w1);
+                        p[h][nb][e][0] = transposed(pair);
+                        if (kWeights == 2) p[h][nb][e][kWeights - 1] = transposed(rest_pair(w0, w1, pair));
+                    }
 
             // values
 #pragma unroll
@@ -636,153 +675,148 @@ k_cache_attend(const __grid_constant__ Attend a) {
         }
 
         // ---- the warps' parts into one
-        const bool whole = place.tile == 0 && n == place.tiles;
-        const int rows = min(kRows, place.s.count * a.group - place.qtile * kRows), live = min(n, WARPS);  // the first `live` warps had units
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float x = l[nb][c];
-#pragma unroll
-                for (int d = 4; d < 32; d *= 2) x += __shfl_xor_sync(0xFFFFFFFFu, x, d);
-                if (g == 0) {
-                    joining.m[8 * nb + 2 * t + c][warp] = m[nb][c];
-                    joining.l[8 * nb + 2 * t + c][warp] = x;
-                }
-            }
         const Place done = place;
-        const int done_units = n;
-        next_segment<kRows>(a, place);
-        if (unit + done_units < to) {  // the next tile's queries and first units, on their way meanwhile
+        const int done_units = n, live = min(n, WARPS);  // the first `live` warps had units
+        const bool whole = done.tile == 0 && n == done.tiles;
+        at_unit += n;
+        if (done.tile + n == done.tiles) at_unit += kSegment;
+        const bool more = at_unit < to;
+        if (more) {  // the next segment's queries and first units, on their way meanwhile
+            next_segment<kRows>(a, place);
             raw.load(a, place);
-            n = min(place.tiles, to - unit - done_units);
+            n = min(place.tiles, to - at_unit);
             my_units = begin(n);
         }
+        if (warp < live) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int r = 8 * nb + 2 * t + c;
+                    float x = l[nb][c];
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) x += __shfl_xor_sync(0xFFFFFFFFu, x, d);
+                    if (g == 0) {
+                        joining.m[r][warp] = m[nb][c];
+                        joining.l[r][warp] = x;
+                    }
+#pragma unroll
+                    for (int k = 0; k < S::kTiles; ++k)
+                        *reinterpret_cast<float2*>(&joining.o[warp][r][joining.at(g * (DIM / 8) + 2 * k)]) = make_float2(o[nb][k][c], o[nb][k][c + 2]);
+#pragma unroll
+                    for (int k = 0; k < S::kBitTiles; ++k) {
+                        joining.bits[warp][r][g * (DIM / 64) + 2 * k] = bits[nb][k][c];
+                        if (DIM > 64) joining.bits[warp][r][g * (DIM / 64) + 2 * k + 1] = bits[nb][k][c + 2];
+                    }
+                }
+        }
+        if (more) raw.put(a, all_queries[buffer ^ 1]);
         __syncthreads();
-        // of row r: the largest maximum of the warps
-        const auto top_of = [&](int r) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) top = w < live ? larger(top, joining.m[r][w]) : top;
-            return top;
-        };
-        const int q_heads = a.group * a.pages.n_heads;
-        // row r of the tile: where its result goes
-        const auto row_of = [&](int r) {
-            const int row = done.qtile * kRows + r;
-            return (int64_t)(done.s.first + row / a.group) * q_heads + done.head * a.group + row % a.group;
-        };
-        const auto put = [&](int r, int d, float x, float y) {
-            if (PARTS == 2) *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + row_of(r) * DIM + d) = __floats2bfloat162_rn(x, y);
-            else *reinterpret_cast<float2*>(static_cast<float*>(a.out) + row_of(r) * DIM + d) = make_float2(x, y);
-        };
-        const auto put_lse = [&](int r, float top, float sum) {
-            if (a.lse) a.lse[row_of(r)] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * 0.69314718f;
-        };
-        // a CTA's parts: of the segment that began before it, and of the one that goes on behind it
-        constexpr int kPart = kRows * (DIM + 2);
+        const int rows = min(kRows, done.s.count * a.group - done.qtile * kRows);
         float* partial = a.partials + ((int64_t)blockIdx.x * 2 + (done.tile > 0 ? 0 : 1)) * kPart;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            if (nb > 0) __syncthreads();  // the tile before is read
-            if (warp < live) {
-                float scale[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) scale[c] = m[nb][c] == -INFINITY ? 0.0f : exp2_of(m[nb][c] - top_of(8 * nb + 2 * t + c));
-#pragma unroll
-                for (int k = 0; k < S::kTiles; ++k) {
-                    const int d = g * (DIM / 8) + 2 * k, block = k / 4;  // of the lane's blocks
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const float half = bits[nb][block / 2][c + 2 * (block & 1)] * (0.5f / of_bit(block));
-                        float2 v = make_float2((o[nb][k][c] + half) * scale[c], (o[nb][k][c + 2] + half) * scale[c]);
-                        if (scale[c] == 0.0f) v = make_float2(0.0f, 0.0f);
-                        *reinterpret_cast<float2*>(&joining.o[warp][2 * t + c][joining.at(d)]) = v;
-                    }
+#pragma unroll 1
+        for (int at = threadIdx.x; at < rows * (DIM / 2); at += kThreads) {
+            const int r = at / (DIM / 2), d = at % (DIM / 2) * 2;
+            float highest = kNothing, sum = 0.0f;
+            for (int w = 0; w < live; ++w) highest = larger(highest, joining.m[r][w]);
+            float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+            for (int w = 0; w < live; ++w) {
+                const float keep = exp2_of(joining.m[r][w] - highest);
+                if (keep != 0.0f) {  // a warp that saw nothing has nothing to add, whatever the row's maximum is
+                    const float2 x = *reinterpret_cast<const float2*>(&joining.o[w][r][joining.at(d)]);
+                    const float half = joining.bits[w][r][d / 8] * half_of_bit<DIM>(d / 8);
+                    v.x += (x.x + half) * keep;
+                    v.y += (x.y + half) * keep;
+                    sum += joining.l[r][w] * keep;
                 }
             }
-            __syncthreads();
-            for (int at = threadIdx.x; at < 8 * DIM / 2; at += kThreads) {
-                const int r = 8 * nb + at / (DIM / 2), d = at % (DIM / 2) * 2;
-                if (r >= rows) continue;
-                float2 v = make_float2(0.0f, 0.0f);
-                const float top = top_of(r);
-                float sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    if (w >= live) break;
-                    const float2 x = *reinterpret_cast<const float2*>(&joining.o[w][r % 8][joining.at(d)]);
-                    v.x += x.x;
-                    v.y += x.y;
-                    const float its = joining.m[r][w], keep = its == -INFINITY ? 0.0f : exp2_of(its - top);
-                    if (keep != 0.0f) sum += joining.l[r][w] * keep;
-                }
-                if (whole) {
-                    put(r, d, top == -INFINITY ? 0.0f : v.x / sum, top == -INFINITY ? 0.0f : v.y / sum);
-                    if (d == 0) put_lse(r, top, sum);
-                } else {
-                    *reinterpret_cast<float2*>(partial + 2 * kRows + r * DIM + d) = v;
-                    if (d == 0) {
-                        partial[r] = top;
-                        partial[kRows + r] = sum;
-                    }
+            if (whole) {
+                const float part_of = highest == kNothing ? 0.0f : 1.0f / sum;
+                put_pair<PARTS, DIM>(a, done, kRows, r, d, v.x * part_of, v.y * part_of);
+                if (d == 0) put_lse(a, done, kRows, r, highest, sum);
+            } else {
+                *reinterpret_cast<float2*>(partial + 2 * kRows + r * DIM + d) = v;
+                if (d == 0) {
+                    partial[r] = highest;
+                    partial[kRows + r] = sum;
                 }
             }
         }
-        // ---- the CTAs' parts into one: those from the CTA with the segment's first unit to the one with its last
         __syncthreads();  // joined, and the parts written
-        if (!whole) {
-            const int first_cta = cut.cta_of(unit - done.tile), parts = cut.cta_of(unit - done.tile + done.tiles - 1) - first_cta + 1;
+        if (!whole) {  // the parts are those of the CTA with the segment's first unit to the one with its last
             if (threadIdx.x == 0) {
-                uint32_t arrived;
-                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(arrived) : "l"(a.counters + first_cta) : "memory");
-                is_last = arrived == (uint32_t)(parts - 1);
+                const int first = at_unit - (done.tile + done_units == done.tiles ? kSegment : 0) - done_units - done.tile;
+                Pending& own = pending[n_pending];
+                own.place = done;
+                own.first_cta = cut.cta_of(first);
+                own.parts = cut.cta_of(first + done.tiles - 1) - own.first_cta + 1;
+                uint32_t before;
+                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + own.first_cta) : "memory");
+                arrived[n_pending] = before;  // looked at in the end: the answer takes its time
             }
-            __syncthreads();
-            if (is_last) {
-                constexpr int kAtOnce = 10;
-                for (int at = threadIdx.x; at < rows * (DIM / 4); at += kThreads) {
-                    const int r = at / (DIM / 4), d = at % (DIM / 4) * 4;
-                    float top = -INFINITY, sum = 0.0f;
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (int i0 = 0; i0 < parts; i0 += kAtOnce) {
-                        float m_of[kAtOnce], l_of[kAtOnce];
-                        float4 x[kAtOnce];
-#pragma unroll
-                        for (int i = 0; i < kAtOnce; ++i) {
-                            const float* part = a.partials + ((int64_t)(first_cta + i0 + i) * 2 + (i0 + i == 0 ? 1 : 0)) * kPart;
-                            m_of[i] = -INFINITY;
-                            if (i0 + i < parts) {
-                                m_of[i] = __ldcg(part + r);
-                                l_of[i] = __ldcg(part + kRows + r);
-                                x[i] = __ldcg(reinterpret_cast<const float4*>(part + 2 * kRows + r * DIM + d));
-                            }
-                        }
-                        float higher = top;
-#pragma unroll
-                        for (int i = 0; i < kAtOnce; ++i) higher = larger(higher, m_of[i]);
-                        const float before = top == -INFINITY ? 0.0f : exp2_of(top - higher);
-                        v.x *= before; v.y *= before; v.z *= before; v.w *= before;
-                        sum *= before;
-                        top = higher;
-#pragma unroll
-                        for (int i = 0; i < kAtOnce; ++i) {
-                            const float keep = m_of[i] == -INFINITY ? 0.0f : exp2_of(m_of[i] - top);
-                            if (keep != 0.0f) {
-                                v.x += x[i].x * keep; v.y += x[i].y * keep; v.z += x[i].z * keep; v.w += x[i].w * keep;
-                                sum += l_of[i] * keep;
-                            }
-                        }
-                    }
-                    const float part_of = top == -INFINITY ? 0.0f : 1.0f / sum;
-                    put(r, d, v.x * part_of, v.y * part_of);
-                    put(r, d + 2, v.z * part_of, v.w * part_of);
-                    if (d == 0) put_lse(r, top, sum);
-                }
-                if (threadIdx.x == 0) a.counters[first_cta] = 0;
+            ++n_pending;
+        }
+        if (!more) break;
+        buffer ^= 1;
+    }
+
+    // ---- the CTAs' parts into one, by the last CTA that has one, in the order of the CTAs
+    if (n_pending > 0) {
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < n_pending; ++i) {
+                pending[i].is_last = arrived[i] == (uint32_t)(pending[i].parts - 1);
+                if (pending[i].is_last) a.counters[pending[i].first_cta] = 0;
             }
         }
-        unit += done_units;
+        __syncthreads();
+#pragma unroll 1
+        for (int i = 0; i < n_pending; ++i) {
+            if (!pending[i].is_last) continue;
+            const Place& done = pending[i].place;
+            const int rows = min(kRows, done.s.count * a.group - done.qtile * kRows), first_cta = pending[i].first_cta, parts = pending[i].parts;
+#pragma unroll 1
+            for (int at = threadIdx.x; at < rows * (DIM / 4); at += kThreads) {
+                const int r = at / (DIM / 4), d = at % (DIM / 4) * 4;
+                float highest = kNothing, sum = 0.0f;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                constexpr int kAtOnce = 8;
+#pragma unroll 1
+                for (int i0 = 0; i0 < parts; i0 += kAtOnce) {
+                    float m_of[kAtOnce], l_of[kAtOnce];
+                    float4 x[kAtOnce];
+#pragma unroll
+                    for (int k = 0; k < kAtOnce; ++k) {
+                        const float* part = a.partials + ((int64_t)(first_cta + i0 + k) * 2 + (i0 + k == 0 ? 1 : 0)) * kPart;
+                        m_of[k] = kNothing;
+                        if (i0 + k < parts) {
+                            m_of[k] = __ldcg(part + r);
+                            l_of[k] = __ldcg(part + kRows + r);
+                            x[k] = __ldcg(reinterpret_cast<const float4*>(part + 2 * kRows + r * DIM + d));
+                        }
+                    }
+                    float higher = highest;
+#pragma unroll
+                    for (int k = 0; k < kAtOnce; ++k) higher = larger(higher, m_of[k]);
+                    const float before = exp2_of(highest - higher);
+                    v.x *= before; v.y *= before; v.z *= before; v.w *= before;
+                    sum *= before;
+                    highest = higher;
+#pragma unroll
+                    for (int k = 0; k < kAtOnce; ++k) {
+                        const float keep = i0 + k < parts ? exp2_of(m_of[k] - highest) : 0.0f;
+                        if (keep != 0.0f) {
+                            v.x += x[k].x * keep; v.y += x[k].y * keep; v.z += x[k].z * keep; v.w += x[k].w * keep;
+                            sum += l_of[k] * keep;
+                        }
+                    }
+                }
+                const float part_of = highest == kNothing ? 0.0f : 1.0f / sum;
+                put_pair<PARTS, DIM>(a, done, kRows, r, d, v.x * part_of, v.y * part_of);
+                put_pair<PARTS, DIM>(a, done, kRows, r, d + 2, v.z * part_of, v.w * part_of);
+                if (d == 0) put_lse(a, done, kRows, r, highest, sum);
+            }
+        }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -790,22 +824,22 @@ k_cache_attend(const __grid_constant__ Attend a) {
 constexpr int kMostRows = 16;
 int64_t scratch_bytes_of(int head_dim) { return 4 * kMostCtas + (int64_t)kMostCtas * 2 * kMostRows * (head_dim + 2) * 4; }
 
-template <int DIM, int PARTS, int NB, int WARPS>
+template <int DIM, int PARTS, int NB, int WARPS, int CTAS>
 int launch_as(const Attend& a, cudaStream_t st) {
     using L = Layout<DIM, PARTS, NB, WARPS>;
-    static_assert(L::kBytes <= 227 * 1024, "shared memory");
+    static_assert(CTAS * (L::kBytes + 1024) <= 228 * 1024, "shared memory");
     static_assert(8 * NB <= kMostRows, "scratch memory");
-    const auto kernel = k_cache_attend<DIM, PARTS, NB, WARPS>;
+    const auto kernel = k_cache_attend<DIM, PARTS, NB, WARPS, CTAS>;
     if (int e = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes), "cudaFuncSetAttribute")) return e;
-    const int sms = sm_count(), grid = sms < kMostCtas ? sms : kMostCtas;
+    const int most = CTAS * sm_count(), grid = most < kMostCtas ? most : kMostCtas;
     return launch_dependent("e8_cache_attention", kernel, (unsigned)grid, 32 * WARPS, L::kBytes, st, a);
 }
 
 template <int DIM, int PARTS>
 int launch(const Attend& a, cudaStream_t st) {
     const int64_t rows = ((int64_t)a.n_queries + a.n_seqs - 1) / a.n_seqs * a.group;  // of a cache head, on average
-    if (rows <= 8) return launch_as<DIM, PARTS, 1, 8>(a, st);
-    return launch_as<DIM, PARTS, 2, DIM == 256 && PARTS == 3 ? 6 : 8>(a, st);
+    if (rows <= 8) return launch_as<DIM, PARTS, 1, DIM == 256 ? 6 : 4, DIM == 256 ? 1 : 2>(a, st);
+    return launch_as<DIM, PARTS, 2, DIM == 256 ? 4 : 4, DIM == 256 ? 1 : 2>(a, st);
 }
 
 }  // namespace
@@ -831,7 +865,7 @@ int coset_e8_cache_attention(const void* q, int dtype, int64_t q_token_stride, i
     if ((int64_t)n_queries * q_heads > INT32_MAX - 64) return fail(COSET_E_UNSUPPORTED, "too many rows for one call");
     if (n_seqs == 0) return 0;
     // no more than this many units are cut among the CTAs, however the queries are shared among the sequences
-    const int64_t tiles = ((int64_t)n_queries * (q_heads / n_heads) + 7) / 8 + n_seqs, longest = ((int64_t)max_pages * page_size + kUnit - 1) / kUnit + 1;
+    const int64_t tiles = ((int64_t)n_queries * (q_heads / n_heads) + 7) / 8 + n_seqs, longest = ((int64_t)max_pages * page_size + kUnit - 1) / kUnit + 1 + kSegment;
     if (n_pages * n_heads >= UINT32_MAX) return fail(COSET_E_UNSUPPORTED, "2^32 or more records");
     if ((double)tiles * n_heads * longest > 2e9) return fail(COSET_E_UNSUPPORTED, "too much work for one call: queries x pages of the table");
     const int64_t whole = dtype == COSET_DTYPE_F32 ? 4 : 8;
