@@ -17,51 +17,90 @@ using namespace coset::cache;
 namespace {
 
 constexpr int kThreads = 256;
+constexpr float kRound = 12582912.0f;  // 1.5 2^23: added to a small number it rounds it to a whole one, which stands in the low bits
+constexpr int kRoundBits = 0x4B400000;
+
+// A thread has a block of 8 values, DIM / 8 neighbours a row; a CTA has rows of one head, one token after the other, so that codes of tokens that
+// share a page are written and read as whole lines.  Rows of a CTA in one round:
+__host__ __device__ constexpr int rows_per_round(int dim) { return kThreads / (dim / 8); }
 
 template <int DT>
-__device__ __forceinline__ void load_block(const void* x, int64_t at, float (&v)[8]);
+struct Block;  // 8 values as they are in memory
 template <>
-__device__ __forceinline__ void load_block<COSET_DTYPE_F32>(const void* x, int64_t at, float (&v)[8]) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at);
-    const float4 a = __ldcs(p), b = __ldcs(p + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <>
-__device__ __forceinline__ void load_block<COSET_DTYPE_BF16>(const void* x, int64_t at, float (&v)[8]) {
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(x) + at));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+struct Block<COSET_DTYPE_F32> {
+    uint4 a, b;
+    __device__ __forceinline__ void load(const void* x, int64_t at) {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(x) + at);
+        a = __ldcs(p);
+        b = __ldcs(p + 1);
     }
-}
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+    }
+    // bits of the largest |value|: ordered like the numbers, infinities and NaN above all
+    __device__ __forceinline__ uint32_t most() const {
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+        return m;
+    }
+};
+template <>
+struct Block<COSET_DTYPE_BF16> {
+    uint4 a;
+    __device__ __forceinline__ void load(const void* x, int64_t at) { a = __ldcs(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(x) + at)); }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+    __device__ __forceinline__ uint32_t most() const {
+        const auto larger = [](uint32_t x, uint32_t y) {
+            uint32_t z;
+            asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
+            return z;
+        };
+        const uint32_t m = larger(larger(a.x & 0x7FFF7FFFu, a.y & 0x7FFF7FFFu), larger(a.z & 0x7FFF7FFFu, a.w & 0x7FFF7FFFu));
+        return max(m << 16, m & 0xFFFF0000u);
+    }
+};
 
-// The code word of the nearest point to u / 4096, and its bit c.
-__device__ __forceinline__ uint32_t nearest_point(const int (&u)[8], bool* half) {
-    int f[8], d[8], sum_f = 0, sum_h = 0, sum_a = 0, top = 0, low = INT32_MAX;
+// The code word of the nearest point to the scaled values x, and its bit c.  y = u + 2048 holds f in the bits from 12 on and d + 2048 below; of the sums of
+// f and of the floors (f, less one where d < 0) only the last bit is wanted, which exclusive-or gives.
+__device__ __forceinline__ uint32_t nearest_point(const float (&x)[8], float inv, bool* half) {
+    int d[8], top = 0, low = INT32_MAX, sum_a = 0;
+    uint32_t odd = 0, negative = 0, word = 0x88888888u, lower = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        f[i] = (u[i] + 2048) >> 12;
-        d[i] = u[i] - (f[i] << 12);
-        const int a = abs(d[i]);
-        sum_f += f[i];
-        sum_h += f[i] - (d[i] < 0);
-        sum_a += a;
-        top = max(top, a * 8 + 7 - i);
-        low = min(low, a * 8 + i);
+        const int y = __float_as_int(__fmaf_rn(__fmul_rn(x[i], inv), kGrid, kRound)) - (kRoundBits - 2048);  // the product with 4096 is exact
+        const int f = y >> 12;
+        d[i] = (y & 4095) - 2048;
+        odd ^= (uint32_t)y;
+        negative ^= (uint32_t)d[i];
+        word += (uint32_t)f << (4 * i);
+        lower += ((uint32_t)d[i] >> 31) << (4 * i);
+        const int key = abs(d[i]) * 8;
+        sum_a += key;
+        top = max(top, key + 7 - i);
+        low = min(low, key + i);
     }
-    const bool odd_f = sum_f & 1, odd_h = sum_h & 1;
-    const int far = odd_f ? 4096 - 2 * (top >> 3) : 0, half_far = 8192 - sum_a + (odd_h ? 2 * (low >> 3) : 0);
+    const bool odd_f = odd >> 12 & 1, odd_h = (odd >> 12 ^ negative >> 31) & 1;
+    const int far = odd_f ? 4096 - 2 * (top >> 3) : 0, half_far = 8192 - (sum_a >> 3) + (odd_h ? 2 * (low >> 3) : 0);
     const bool c = half_far < far;
-    const int moved = c ? (odd_h ? low & 7 : 8) : (odd_f ? 7 - (top & 7) : 8);
-    uint32_t word = 0;
+    // the coordinate that moves: away from the whole number towards the value, and the other way round from the half-odd one
+    const int k = c ? low & 7 : 7 - (top & 7);
+    int its = d[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int whole = f[i] + (i == moved ? (d[i] > 0 ? 1 : -1) : 0);
-        const int halved = f[i] - (d[i] < 0) + (i == moved ? (d[i] < 0 && d[i] > -2048 ? 1 : -1) : 0);
-        word |= (uint32_t)((c ? halved : whole) + 8) << (4 * i);
-    }
+    for (int i = 1; i < 8; ++i) its = i == k ? d[i] : its;
+    const bool up = c ? its < 0 && its > -2048 : its > 0;
+    if (c) word -= lower;
+    if (c ? odd_h : odd_f) word += (up ? 1u : 0xFFFFFFFFu) << (4 * k);
     *half = c;
     return word;
 }
@@ -71,50 +110,55 @@ struct Write {
     const void* x[2];
     int64_t token_stride[2], head_stride[2];
     const int64_t* slots;
-    int64_t n_rows;  // tokens x 2 x heads
+    int64_t n_tokens;
 };
 
-// A thread has a block, DIM / 8 neighbours a row.
-template <int DIM, int DT>
+template <int DIM, int DT, int ROUNDS>
 __global__ void __launch_bounds__(kThreads)
 k_cache_write(const __grid_constant__ Write w) {
-    constexpr int kBlocks = DIM / 8;
+    constexpr int kBlocks = DIM / 8, kRows = rows_per_round(DIM);
     grid_wait();
     grid_trigger();
-    const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    const int64_t row = id / kBlocks;
-    const int b = (int)(id % kBlocks), lane = threadIdx.x & 31;
-    const int pair = (int)(row % (2 * w.pages.n_heads)), which = pair >= w.pages.n_heads, head = pair - which * w.pages.n_heads;
-    const int64_t token = row / (2 * w.pages.n_heads);
-    const int64_t slot = row < w.n_rows ? __ldg(behind_wait(w.slots) + token) : -1;
-    const bool real = slot >= 0 && slot >> w.pages.page_log2 < w.pages.n_pages;
-    float x[8];
+    const int b = threadIdx.x % kBlocks, lane = threadIdx.x & 31, which = blockIdx.y >= w.pages.n_heads, head = blockIdx.y - which * w.pages.n_heads;
+    const int64_t token0 = (int64_t)blockIdx.x * (kRows * ROUNDS) + threadIdx.x / kBlocks;
+    const void* x = (which ? w.x[1] : w.x[0]);
+    const int64_t stride = which ? w.token_stride[1] : w.token_stride[0], first = head * (which ? w.head_stride[1] : w.head_stride[0]) + 8 * b;
+    int64_t slot[ROUNDS];
+    Block<DT> raw[ROUNDS];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    if (real) load_block<DT>(w.x[which], token * w.token_stride[which] + head * w.head_stride[which] + 8 * b, x);
-    uint32_t most = 0;  // of the bits of |x|: ordered like the numbers, infinities and NaN above all
+    for (int i = 0; i < ROUNDS; ++i) slot[i] = token0 + i * kRows < w.n_tokens ? __ldg(behind_wait(w.slots) + token0 + i * kRows) : -1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    for (int i = 0; i < ROUNDS; ++i) {
+        if (slot[i] < 0 || slot[i] >> w.pages.page_log2 >= w.pages.n_pages) slot[i] = -1;
+        raw[i] = {};
+        if (slot[i] >= 0) raw[i].load(x, (token0 + i * kRows) * stride + first);
+    }
 #pragma unroll
-    for (int m = 1; m < kBlocks; m *= 2) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, m));
-    const bool plain = most >= kSmallest && most < 0x7F800000u;
-    uint32_t step = 0x3F800000u;
-    if (plain) step = (__float_as_uint(__fdiv_rn(__uint_as_float(most), kLevels)) + 0xFFFFu) & 0xFFFF0000u;
-    const float inv = __fdiv_rn(1.0f, __uint_as_float(step));
-    int u[8];
+    for (int i = 0; i < ROUNDS; ++i) {
+        uint32_t most = raw[i].most();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] = plain ? __float2int_rn(__fmul_rn(__fmul_rn(x[i], inv), kGrid)) : 0;
-    bool half;
-    const uint32_t word = nearest_point(u, &half);
-    const uint32_t votes = __ballot_sync(0xFFFFFFFFu, half);
-    if (!real) return;
-    if (!plain) step = most < kSmallest ? 0u : kNoNumber;
-    const int at = (int)(slot & ((1 << w.pages.page_log2) - 1));
-    uint32_t* rec = w.pages.words + record<DIM>(w.pages, slot >> w.pages.page_log2, head);
-    rec[(((which << w.pages.page_log2) + at)) * kBlocks + b] = word;
-    if (b < head_words(DIM)) {
-        const uint32_t mine = votes >> (lane - b + 16 * b);
-        rec[((2 * kBlocks + which * head_words(DIM)) << w.pages.page_log2) + at * head_words(DIM) + b] = step | (mine & (kBlocks < 16 ? 0xFFu : 0xFFFFu));
+        for (int m = 1; m < kBlocks; m *= 2) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, m));
+        const bool plain = most >= kSmallest && most < 0x7F800000u;
+        uint32_t step = 0x3F800000u;
+        if (plain) step = (__float_as_uint(__fdiv_rn(__uint_as_float(most), kLevels)) + 0xFFFFu) & 0xFFFF0000u;
+        float v[8];
+        raw[i].values(v);
+        if (!plain) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+        }
+        bool half;
+        const uint32_t word = nearest_point(v, __fdiv_rn(1.0f, __uint_as_float(step)), &half);
+        const uint32_t votes = __ballot_sync(0xFFFFFFFFu, half);
+        if (slot[i] < 0) continue;
+        if (!plain) step = most < kSmallest ? 0u : kNoNumber;
+        const int at = (int)slot[i] & ((1 << w.pages.page_log2) - 1);
+        uint32_t* rec = w.pages.words + record<DIM>(w.pages, slot[i] >> w.pages.page_log2, head);
+        rec[((which << w.pages.page_log2) + at) * kBlocks + b] = word;
+        if (b < head_words(DIM)) {
+            const uint32_t mine = votes >> (lane - b + 16 * b);
+            rec[((2 * kBlocks + which * head_words(DIM)) << w.pages.page_log2) + at * head_words(DIM) + b] = step | (mine & (kBlocks < 16 ? 0xFFu : 0xFFFFu));
+        }
     }
 }
 
@@ -122,66 +166,94 @@ struct Read {
     Pages pages;
     void* out[2];
     const int64_t* slots;
-    int64_t n_rows;
+    int64_t n_tokens;
 };
 
-template <int DIM, int DT>
+template <int DIM, int DT, int ROUNDS>
 __global__ void __launch_bounds__(kThreads)
 k_cache_read(const __grid_constant__ Read r) {
-    constexpr int kBlocks = DIM / 8;
+    constexpr int kBlocks = DIM / 8, kRows = rows_per_round(DIM);
     grid_wait();
     grid_trigger();
-    const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    const int64_t row = id / kBlocks;
-    if (row >= r.n_rows) return;
-    const int b = (int)(id % kBlocks);
-    const int pair = (int)(row % (2 * r.pages.n_heads)), which = pair >= r.pages.n_heads, head = pair - which * r.pages.n_heads;
-    const int64_t token = row / (2 * r.pages.n_heads);
-    const int64_t slot = __ldg(behind_wait(r.slots) + token);
-    float v[8];
+    const int b = threadIdx.x % kBlocks, which = blockIdx.y >= r.pages.n_heads, head = blockIdx.y - which * r.pages.n_heads;
+    const int64_t token0 = (int64_t)blockIdx.x * (kRows * ROUNDS) + threadIdx.x / kBlocks;
+    int64_t slot[ROUNDS];
+    uint32_t word[ROUNDS], top[ROUNDS];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    if (slot >= 0 && slot >> r.pages.page_log2 < r.pages.n_pages) {
-        const int at = (int)(slot & ((1 << r.pages.page_log2) - 1));
-        const uint32_t* rec = r.pages.words + record<DIM>(r.pages, slot >> r.pages.page_log2, head);
-        const uint32_t word = rec[((which << r.pages.page_log2) + at) * kBlocks + b];
-        const uint32_t h = rec[((2 * kBlocks + which * head_words(DIM)) << r.pages.page_log2) + at * head_words(DIM) + b / 16];
-        const float step = __uint_as_float(h & 0xFFFF0000u), c = (h >> (b % 16)) & 1 ? -7.5f : -8.0f;
+    for (int i = 0; i < ROUNDS; ++i) slot[i] = token0 + i * kRows < r.n_tokens ? __ldg(behind_wait(r.slots) + token0 + i * kRows) : -1;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn((float)((word >> (4 * i)) & 15u) + c, step);
-    }
-    const int64_t to = (token * r.pages.n_heads + head) * DIM + 8 * b;
-    if (DT == COSET_DTYPE_F32) {
-        float4* p = reinterpret_cast<float4*>(static_cast<float*>(r.out[which]) + to);
-        __stcs(p, make_float4(v[0], v[1], v[2], v[3]));
-        __stcs(p + 1, make_float4(v[4], v[5], v[6], v[7]));
-    } else {
-        uint32_t o[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 h2 = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-            o[i] = *reinterpret_cast<const uint32_t*>(&h2);
+    for (int i = 0; i < ROUNDS; ++i) {
+        word[i] = 0x88888888u;
+        top[i] = 0;
+        if (slot[i] >= 0 && slot[i] >> r.pages.page_log2 < r.pages.n_pages) {
+            const int at = (int)slot[i] & ((1 << r.pages.page_log2) - 1);
+            const uint32_t* rec = r.pages.words + record<DIM>(r.pages, slot[i] >> r.pages.page_log2, head);
+            word[i] = rec[((which << r.pages.page_log2) + at) * kBlocks + b];
+            top[i] = rec[((2 * kBlocks + which * head_words(DIM)) << r.pages.page_log2) + at * head_words(DIM) + b / 16];
         }
-        __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(r.out[which]) + to), make_uint4(o[0], o[1], o[2], o[3]));
+    }
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+        if (token0 + i * kRows >= r.n_tokens) continue;
+        // a nibble at bits 1..4 under the exponent of 2^22 is the number 2^22 + n
+        const float step = __uint_as_float(top[i] & 0xFFFF0000u), less = top[i] >> (b % 16) & 1 ? 4194311.5f : 4194312.0f;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t shifted = k == 0 ? word[i] << 1 : word[i] >> (4 * k - 1);
+            v[k] = __fmul_rn(__uint_as_float((shifted & 0x1Eu) | 0x4A800000u) - less, step);
+        }
+        const int64_t to = ((token0 + i * kRows) * r.pages.n_heads + head) * DIM + 8 * b;
+        void* out = which ? r.out[1] : r.out[0];
+        if (DT == COSET_DTYPE_F32) {
+            float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + to);
+            __stcs(p, make_float4(v[0], v[1], v[2], v[3]));
+            __stcs(p + 1, make_float4(v[4], v[5], v[6], v[7]));
+        } else {
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const __nv_bfloat162 h2 = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+                o[k] = *reinterpret_cast<const uint32_t*>(&h2);
+            }
+            __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to), make_uint4(o[0], o[1], o[2], o[3]));
+        }
     }
 }
 
-// Blocks of a launch over n_rows rows of `dim` values; -1: more than a grid holds.
-int64_t grid_of(int64_t n_rows, int dim) {
-    const int64_t per = kThreads / (dim / 8), need = (n_rows + per - 1) / per;
-    return need > INT32_MAX ? -1 : need;
-}
 bool known_dtype(int dtype) { return dtype == COSET_DTYPE_F32 || dtype == COSET_DTYPE_BF16; }
 
-template <int DIM>
-int launch_write(const Write& w, int dtype, unsigned grid, cudaStream_t st) {
-    return dtype == COSET_DTYPE_F32 ? launch_dependent("e8_cache_write", k_cache_write<DIM, COSET_DTYPE_F32>, grid, kThreads, 0, st, w)
-                                    : launch_dependent("e8_cache_write", k_cache_write<DIM, COSET_DTYPE_BF16>, grid, kThreads, 0, st, w);
+// The grid of a call, and whether its CTAs do four rounds: from four CTAs per SM on.
+struct Shape {
+    dim3 grid;
+    bool many;
+};
+int shape_of(int64_t n_tokens, int n_heads, int dim, Shape* s) {
+    const int64_t rows = rows_per_round(dim), once = (n_tokens + rows - 1) / rows;
+    s->many = once * 2 * n_heads >= 16 * (int64_t)sm_count();
+    const int64_t x = s->many ? (once + 3) / 4 : once;
+    if (x > INT32_MAX) return fail(COSET_E_UNSUPPORTED, "too many tokens for one call");
+    s->grid = dim3((unsigned)x, 2 * (unsigned)n_heads);
+    return 0;
+}
+
+template <int DIM, int DT>
+int launch_write(const Write& w, const Shape& s, cudaStream_t st) {
+    return s.many ? launch_dependent("e8_cache_write", k_cache_write<DIM, DT, 4>, s.grid, kThreads, 0, st, w)
+                  : launch_dependent("e8_cache_write", k_cache_write<DIM, DT, 1>, s.grid, kThreads, 0, st, w);
+}
+template <int DIM, int DT>
+int launch_read(const Read& r, const Shape& s, cudaStream_t st) {
+    return s.many ? launch_dependent("e8_cache_read", k_cache_read<DIM, DT, 4>, s.grid, kThreads, 0, st, r)
+                  : launch_dependent("e8_cache_read", k_cache_read<DIM, DT, 1>, s.grid, kThreads, 0, st, r);
 }
 template <int DIM>
-int launch_read(const Read& r, int dtype, unsigned grid, cudaStream_t st) {
-    return dtype == COSET_DTYPE_F32 ? launch_dependent("e8_cache_read", k_cache_read<DIM, COSET_DTYPE_F32>, grid, kThreads, 0, st, r)
-                                    : launch_dependent("e8_cache_read", k_cache_read<DIM, COSET_DTYPE_BF16>, grid, kThreads, 0, st, r);
+int launch_write(const Write& w, int dtype, const Shape& s, cudaStream_t st) {
+    return dtype == COSET_DTYPE_F32 ? launch_write<DIM, COSET_DTYPE_F32>(w, s, st) : launch_write<DIM, COSET_DTYPE_BF16>(w, s, st);
+}
+template <int DIM>
+int launch_read(const Read& r, int dtype, const Shape& s, cudaStream_t st) {
+    return dtype == COSET_DTYPE_F32 ? launch_read<DIM, COSET_DTYPE_F32>(r, s, st) : launch_read<DIM, COSET_DTYPE_BF16>(r, s, st);
 }
 
 }  // namespace
@@ -206,13 +278,11 @@ int coset_e8_cache_write(void* pages, int64_t n_pages, int n_heads, int page_siz
     w.token_stride[0] = k_token_stride; w.token_stride[1] = v_token_stride;
     w.head_stride[0] = k_head_stride; w.head_stride[1] = v_head_stride;
     w.slots = slots;
-    if (n_tokens > INT64_MAX / (2 * (int64_t)n_heads)) return fail(COSET_E_UNSUPPORTED, "too many rows for one call");
-    w.n_rows = n_tokens * 2 * n_heads;
-    const int64_t grid = grid_of(w.n_rows, head_dim);
-    if (grid < 0) return fail(COSET_E_UNSUPPORTED, "too many rows for one call");
+    w.n_tokens = n_tokens;
+    Shape shape;
+    if (int e = shape_of(n_tokens, n_heads, head_dim, &shape)) return e;
     cudaStream_t st = (cudaStream_t)stream;
-    return head_dim == 64 ? launch_write<64>(w, dtype, (unsigned)grid, st) : head_dim == 128 ? launch_write<128>(w, dtype, (unsigned)grid, st)
-                                                                            : launch_write<256>(w, dtype, (unsigned)grid, st);
+    return head_dim == 64 ? launch_write<64>(w, dtype, shape, st) : head_dim == 128 ? launch_write<128>(w, dtype, shape, st) : launch_write<256>(w, dtype, shape, st);
 }
 
 int coset_e8_cache_read(const void* pages, int64_t n_pages, int n_heads, int page_size, int head_dim, const int64_t* slots, int64_t n_tokens,
@@ -226,13 +296,11 @@ int coset_e8_cache_read(const void* pages, int64_t n_pages, int n_heads, int pag
     if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 8)) return fail(COSET_E_ALIGN, "k and v must be 16-byte, slots 8-byte aligned");
     r.out[0] = k; r.out[1] = v;
     r.slots = slots;
-    if (n_tokens > INT64_MAX / (2 * (int64_t)n_heads)) return fail(COSET_E_UNSUPPORTED, "too many rows for one call");
-    r.n_rows = n_tokens * 2 * n_heads;
-    const int64_t grid = grid_of(r.n_rows, head_dim);
-    if (grid < 0) return fail(COSET_E_UNSUPPORTED, "too many rows for one call");
+    r.n_tokens = n_tokens;
+    Shape shape;
+    if (int e = shape_of(n_tokens, n_heads, head_dim, &shape)) return e;
     cudaStream_t st = (cudaStream_t)stream;
-    return head_dim == 64 ? launch_read<64>(r, dtype, (unsigned)grid, st) : head_dim == 128 ? launch_read<128>(r, dtype, (unsigned)grid, st)
-                                                                           : launch_read<256>(r, dtype, (unsigned)grid, st);
+    return head_dim == 64 ? launch_read<64>(r, dtype, shape, st) : head_dim == 128 ? launch_read<128>(r, dtype, shape, st) : launch_read<256>(r, dtype, shape, st);
 }
 
 }  // extern "C"

@@ -39,7 +39,7 @@ inline bool known_dim(int dim) { return dim == 64 || dim == 128 || dim == 256; }
 inline int check_pages(const void* pages, int64_t n_pages, int n_heads, int page_size, int head_dim, Pages* out) {
     if (!known_dim(head_dim)) return fail(COSET_E_UNSUPPORTED, "head_dim must be 64, 128 or 256, got %d", head_dim);
     if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return fail(COSET_E_UNSUPPORTED, "page_size must be a power of two from 16 to 1024, got %d", page_size);
-    if (n_heads < 1 || n_heads > 65535) return fail(COSET_E_BADARG, "n_heads must lie in [1, 65535], got %d", n_heads);
+    if (n_heads < 1 || n_heads > 32767) return fail(COSET_E_BADARG, "n_heads must lie in [1, 32767], got %d", n_heads);
     if (n_pages < 0 || n_pages > INT32_MAX) return fail(COSET_E_BADARG, "n_pages must lie in [0, 2^31), got %lld", (long long)n_pages);
     if (n_pages > 0 && !pages) return fail(COSET_E_BADARG, "pages is null");
     if (!aligned(pages, 16)) return fail(COSET_E_ALIGN, "pages must be 16-byte aligned");

@@ -768,7 +768,7 @@ CachePages pages_arg(PyObject* o) {
     for (int d : {64, 128, 256})
         if (t.size(3) == coset_e8_cache_row_words(d)) dim = d;
     TORCH_CHECK_VALUE(dim != 0, "pages has rows of ", t.size(3), " words, which are those of no head_dim (64, 128 or 256)");
-    TORCH_CHECK_VALUE(t.size(1) >= 1 && t.size(1) <= 65535 && t.size(2) <= 1024 && t.size(0) <= INT32_MAX, "pages has sizes out of range: ", t.sizes());
+    TORCH_CHECK_VALUE(t.size(1) >= 1 && t.size(1) <= 32767 && t.size(2) <= 1024 && t.size(0) <= INT32_MAX, "pages has sizes out of range: ", t.sizes());
     return {t, t.size(0), (int)t.size(1), (int)t.size(2), dim};
 }
 void same_device(const Tensor& t, const Tensor& as, const char* name) {
