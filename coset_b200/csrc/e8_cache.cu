@@ -17,8 +17,7 @@ using namespace coset::cache;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kRound = 12582912.0f;  // 1.5 2^23: added to a small number it rounds it to a whole one, which stands in the low bits
-constexpr int kRoundBits = 0x4B400000;
+constexpr float kRound = 12582912.0f;  // 1.5 2^23: added to a small number it rounds it to a whole one, which stands in the low 22 bits
 
 // A thread has a block of 8 values, DIM / 8 neighbours a row; a CTA has rows of one head, one token after the other, so that codes of tokens that
 // share a page are written and read as whole lines.  Rows of a CTA in one round:
@@ -71,38 +70,47 @@ struct Block<COSET_DTYPE_BF16> {
     }
 };
 
-// The code word of the nearest point to the scaled values x, and its bit c.  y = u + 2048 holds f in the bits from 12 on and d + 2048 below; of the sums of
-// f and of the floors (f, less one where d < 0) only the last bit is wanted, which exclusive-or gives.
+// The code word of the nearest point to the scaled values x, and its bit c.  The bits of u + 1.5 2^23 hold u: its low 12, with their sign, are d, and bit 12 is
+// the last one of floor(u / 4096).  Of the sums of the floors and of f (the floor, and one more where d < 0) only the last bits are wanted, which
+// exclusive-or gives.
 __device__ __forceinline__ uint32_t nearest_point(const float (&x)[8], float inv, bool* half) {
-    int d[8], top = 0, low = INT32_MAX, sum_a = 0;
-    uint32_t odd = 0, negative = 0, word = 0x88888888u, lower = 0;
+    int u[8], d[8], top = 0, low = INT32_MAX, sum_a = 0;
+    uint32_t floors = 0, negative = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int y = __float_as_int(__fmaf_rn(__fmul_rn(x[i], inv), kGrid, kRound)) - (kRoundBits - 2048);  // the product with 4096 is exact
-        const int f = y >> 12;
-        d[i] = (y & 4095) - 2048;
-        odd ^= (uint32_t)y;
+        u[i] = __float_as_int(__fmaf_rn(__fmul_rn(x[i], inv), kGrid, kRound));  // the product with 4096 is exact
+        d[i] = u[i] << 20 >> 20;
+        floors ^= (uint32_t)u[i];
         negative ^= (uint32_t)d[i];
-        word += (uint32_t)f << (4 * i);
-        lower += ((uint32_t)d[i] >> 31) << (4 * i);
-        const int key = abs(d[i]) * 8;
-        sum_a += key;
-        top = max(top, key + 7 - i);
-        low = min(low, key + i);
+        const int a = abs(d[i]);
+        sum_a += a;
+        top = max(top, a * 8 + 7 - i);
+        low = min(low, a * 8 + i);
     }
-    const bool odd_f = odd >> 12 & 1, odd_h = (odd >> 12 ^ negative >> 31) & 1;
-    const int far = odd_f ? 4096 - 2 * (top >> 3) : 0, half_far = 8192 - (sum_a >> 3) + (odd_h ? 2 * (low >> 3) : 0);
+    const bool odd_h = floors >> 12 & 1, odd_f = (floors >> 12 ^ negative >> 31) & 1;
+    const int far = odd_f ? 4096 - 2 * (top >> 3) : 0, half_far = 8192 - sum_a + (odd_h ? 2 * (low >> 3) : 0);
     const bool c = half_far < far;
-    // the coordinate that moves: away from the whole number towards the value, and the other way round from the half-odd one
-    const int k = c ? low & 7 : 7 - (top & 7);
-    int its = d[0];
+    const int offset = c ? 8 * 4096 : 8 * 4096 + 2048;  // to the nibble f + 8 at bits 12..15
+    uint32_t word = 0;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) its = i == k ? d[i] : its;
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t y = (uint32_t)(u[i] + offset);
+        word |= (i < 3 ? y >> (12 - 4 * i) : y << (4 * i - 12)) & (15u << (4 * i));
+    }
+    // the coordinate that moves: from the whole number towards the value, and from the half-odd one
+    const int k = c ? low & 7 : 7 - (top & 7);
+    const int d01 = k & 1 ? d[1] : d[0], d23 = k & 1 ? d[3] : d[2], d45 = k & 1 ? d[5] : d[4], d67 = k & 1 ? d[7] : d[6];
+    const int d03 = k & 2 ? d23 : d01, d47 = k & 2 ? d67 : d45, its = k & 4 ? d47 : d03;
     const bool up = c ? its < 0 && its > -2048 : its > 0;
-    if (c) word -= lower;
     if (c ? odd_h : odd_f) word += (up ? 1u : 0xFFFFFFFFu) << (4 * k);
     *half = c;
     return word;
+}
+
+// x / 7, correctly rounded: the quotient by the rounded reciprocal, corrected by what it leaves (Markstein, 1990); checked for every significand
+__device__ __forceinline__ float seventh(float x) {
+    const float r = 1.0f / 7.0f, q = __fmul_rn(x, r);
+    return __fmaf_rn(__fmaf_rn(-q, kLevels, x), r, q);
 }
 
 struct Write {
@@ -140,7 +148,7 @@ k_cache_write(const __grid_constant__ Write w) {
         for (int m = 1; m < kBlocks; m *= 2) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, m));
         const bool plain = most >= kSmallest && most < 0x7F800000u;
         uint32_t step = 0x3F800000u;
-        if (plain) step = (__float_as_uint(__fdiv_rn(__uint_as_float(most), kLevels)) + 0xFFFFu) & 0xFFFF0000u;
+        if (plain) step = (__float_as_uint(seventh(__uint_as_float(most))) + 0xFFFFu) & 0xFFFF0000u;
         float v[8];
         raw[i].values(v);
         if (!plain) {
@@ -148,7 +156,7 @@ k_cache_write(const __grid_constant__ Write w) {
             for (int k = 0; k < 8; ++k) v[k] = 0.0f;
         }
         bool half;
-        const uint32_t word = nearest_point(v, __fdiv_rn(1.0f, __uint_as_float(step)), &half);
+        const uint32_t word = nearest_point(v, __frcp_rn(__uint_as_float(step)), &half);
         const uint32_t votes = __ballot_sync(0xFFFFFFFFu, half);
         if (slot[i] < 0) continue;
         if (!plain) step = most < kSmallest ? 0u : kNoNumber;
@@ -160,6 +168,13 @@ k_cache_write(const __grid_constant__ Write w) {
             rec[((2 * kBlocks + which * head_words(DIM)) << w.pages.page_log2) + at * head_words(DIM) + b] = step | (mine & (kBlocks < 16 ? 0xFFu : 0xFFFFu));
         }
     }
+}
+
+// (x & mask) | bits in one instruction, of which the compiler makes two when it knows both constants
+__device__ __forceinline__ uint32_t chosen(uint32_t x, uint32_t mask, uint32_t bits) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "r"(mask), "r"(bits));
+    return d;
 }
 
 struct Read {
@@ -195,28 +210,32 @@ k_cache_read(const __grid_constant__ Read r) {
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
         if (token0 + i * kRows >= r.n_tokens) continue;
-        // a nibble at bits 1..4 under the exponent of 2^22 is the number 2^22 + n
-        const float step = __uint_as_float(top[i] & 0xFFFF0000u), less = top[i] >> (b % 16) & 1 ? 4194311.5f : 4194312.0f;
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint32_t shifted = k == 0 ? word[i] << 1 : word[i] >> (4 * k - 1);
-            v[k] = __fmul_rn(__uint_as_float((shifted & 0x1Eu) | 0x4A800000u) - less, step);
-        }
         const int64_t to = ((token0 + i * kRows) * r.pages.n_heads + head) * DIM + 8 * b;
         void* out = which ? r.out[1] : r.out[0];
+        const uint32_t c = top[i] >> (b % 16) & 1;
         if (DT == COSET_DTYPE_F32) {
+            // a nibble at bits 1..4 under the exponent of 2^22, and c at bit 0, is the number 2^22 + n + c / 2
+            const float step = __uint_as_float(top[i] & 0xFFFF0000u);
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t shifted = k == 0 ? word[i] << 1 : word[i] >> (4 * k - 1);
+                v[k] = __fmul_rn(__uint_as_float(chosen(shifted, 0x1Eu, 0x4A800000u | c)) - 4194312.0f, step);
+            }
             float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + to);
             __stcs(p, make_float4(v[0], v[1], v[2], v[3]));
             __stcs(p + 1, make_float4(v[4], v[5], v[6], v[7]));
         } else {
-            uint32_t o[4];
+            // the same in bf16, two at a time: 64 + n + c / 2, less 72; the product with the step is rounded once, as the float32 product would be
+            const uint32_t exponent = 0x42804280u | c * 0x00010001u, step = __byte_perm(top[i], 0, 0x3232);
+            uint32_t v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const __nv_bfloat162 h2 = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-                o[k] = *reinterpret_cast<const uint32_t*>(&h2);
+            for (int k = 0; k < 4; ++k) {  // values k and k + 4
+                const uint32_t shifted = k == 0 ? word[i] << 1 : word[i] >> (4 * k - 1);
+                asm("{\n\t.reg .b32 t;\n\tadd.rn.bf16x2 t, %1, %2;\n\tmul.rn.bf16x2 %0, t, %3;\n\t}" : "=r"(v[k]) : "r"(chosen(shifted, 0x001E001Eu, exponent)), "r"(0xC290C290u), "r"(step));
             }
-            __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to), make_uint4(o[0], o[1], o[2], o[3]));
+            __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to),
+                   make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)));
         }
     }
 }
