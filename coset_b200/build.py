@@ -37,6 +37,7 @@ SOURCES = [
     "f32_product.cu",
     "e8_cache.cu",
     "e8_cache_attention.cu",
+    "e8_cache_attention_many.cu",
     "d4.cu",
 ]
 

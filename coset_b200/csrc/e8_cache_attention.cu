@@ -33,11 +33,7 @@ namespace {
 
 constexpr int kUnit = 32;         // tokens of a warp's step
 constexpr int kLeastUnits = 4;    // of a CTA
-constexpr int kLeastSize = -90;   // exponent of a value's step as far as the running maximum goes: sums of p / 2^kLeastSize stay finite
-constexpr int kMostCtas = 304;    // counters in the scratch memory
 constexpr int kExact = 0x4B400000;  // the bits of kExactly = 1.5 2^23; a whole number of up to 22 bits added to them is added to it
-constexpr float kExactly = 12582912.0f;
-constexpr float kNothing = -3.402823466e38f;  // running maximum of a row that has seen nothing
 // What a segment costs a CTA beyond its units, in units: its queries, its first loads' latency, its joining.  The cut counts it.
 constexpr int kSegment = 16;
 
@@ -82,11 +78,6 @@ struct Exponents {
         asm volatile("mov.b32 %0, 0x64006400;" : "=r"(even));
         asm volatile("mov.b32 %0, 0x54005400;" : "=r"(odd));
     }
-    static __device__ __forceinline__ uint32_t chosen(uint32_t x, uint32_t mask, uint32_t exponent) {
-        uint32_t d;
-        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "r"(mask), "r"(exponent));  // (x & mask) | exponent
-        return d;
-    }
     __device__ __forceinline__ uint32_t even_values(uint32_t x) const {
         uint32_t d;
         asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(chosen(x, 0x000F000Fu, even)), "r"(0xE408E408u));
@@ -102,21 +93,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a) {
     uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
-}
-__device__ __forceinline__ float exp2_of(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// The larger one; not a number where one of them is none.
-__device__ __forceinline__ float larger(float x, float y) {
-    float z;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
-    return z;
-}
-__device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint32_t rest_pair(float lo, float hi, uint32_t pair) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
@@ -161,16 +137,6 @@ struct Joining {
     static __device__ __forceinline__ int at(int d) { return d + 2 * (d / 16); }
 };
 
-// A place in the CTA's row of units: tile `tile` of `tiles` of (seq, head, query tile).
-struct Place {
-    Sequence s;
-    int seq, head, qtile, qtiles, tile, tiles;
-};
-// A segment that other CTAs have parts of, to be joined by the last of them
-struct Pending {
-    Place place;
-    int first_cta, parts, slot, is_last;
-};
 template <int DIM, int PARTS, int NB, int WARPS>
 struct Layout {
     static constexpr int kStages = DIM == 256 ? 2 : 3;
@@ -178,35 +144,6 @@ struct Layout {
     static constexpr int kJoining = kQueries + 2 * (int)sizeof(Queries<DIM, PARTS, NB>);
     static constexpr int kPending = kJoining + (int)sizeof(Joining<DIM, NB, WARPS>);
     static constexpr int kBytes = kPending + 2 * (int)sizeof(Pending);
-};
-
-template <int ROWS>
-__device__ __forceinline__ void enter(const Attend& a, Place& p) {
-    p.s = sequence(a, p.seq);
-    p.qtiles = (p.s.count * a.group + ROWS - 1) / ROWS;
-    p.tiles = max((p.s.len + kUnit - 1) / kUnit, 1);
-}
-template <int ROWS>
-__device__ __forceinline__ void next_segment(const Attend& a, Place& p) {
-    p.tile = 0;
-    if (++p.qtile < p.qtiles) return;
-    p.qtile = 0;
-    if (++p.head < a.pages.n_heads) return;
-    p.head = 0;
-    do {
-        if (++p.seq >= a.n_seqs) return;
-        enter<ROWS>(a, p);
-    } while (p.qtiles == 0);
-}
-
-// The cut of all segments, each as long as its units and kSegment: CTA c has base of that, and one more where c < more.
-struct Cut {
-    int base, more;
-    __device__ __forceinline__ int from(int cta) const { return base * cta + min(cta, more); }
-    __device__ __forceinline__ int cta_of(int at) const {
-        const int longer = more * (base + 1);
-        return at < longer ? at / (base + 1) : more + (at - longer) / base;
-    }
 };
 
 // A thread's part of a tile of queries on its way to shared memory: blocks of 8 values of rows, whole warps at a time.
@@ -300,21 +237,6 @@ struct QueryBlocks {
 // Half a block's bit, from the sum over what the bit stands for as a 16-bit number
 template <int DIM>
 __device__ __forceinline__ float half_of_bit(int block) { return 0.5f / of_bit(block % (DIM / 64)); }
-// Row r of a tile of `rows` queries: where its result goes
-__device__ __forceinline__ int64_t result_row(const Attend& a, const Place& p, int rows, int r) {
-    const int row = p.qtile * rows + r, query = row / a.group;
-    return (int64_t)(p.s.first + query) * (a.group * a.pages.n_heads) + p.head * a.group + row - query * a.group;
-}
-template <int PARTS, int DIM>
-__device__ __forceinline__ void put_pair(const Attend& a, const Place& p, int rows, int r, int d, float x, float y) {
-    const int64_t at = result_row(a, p, rows, r) * DIM + d;
-    if (PARTS == 2) *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + at) = __floats2bfloat162_rn(x, y);
-    else *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(x, y);
-}
-__device__ __forceinline__ void put_lse(const Attend& a, const Place& p, int rows, int r, float highest, float sum) {
-    if (a.lse) a.lse[result_row(a, p, rows, r)] = highest == kNothing ? -INFINITY : (highest + log2f(sum)) * 0.69314718f;
-}
-
 template <int DIM, int PARTS, int NB, int WARPS, int CTAS>
 __global__ void __launch_bounds__(32 * WARPS, CTAS)
 k_cache_attend(const __grid_constant__ Attend a) {
@@ -331,59 +253,12 @@ k_cache_attend(const __grid_constant__ Attend a) {
     grid_wait();
     grid_trigger();
 
-    // ---- this CTA's units; every warp finds them by itself
-    Place place;
-    const auto units_of = [&](int b) {
-        place.s.count = 0;
-        if (b >= a.n_seqs) return (int64_t)0;
-        place.seq = b;
-        enter<kRows>(a, place);
-        return (int64_t)place.qtiles * a.pages.n_heads * (place.tiles + kSegment);
-    };
-    const auto inclusive = [&](int64_t v) {
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const int64_t u = __shfl_up_sync(0xFFFFFFFFu, v, d);
-            if (lane >= d) v += u;
-        }
-        return v;
-    };
-    int64_t all = 0;
-    for (int b = 32; b < a.n_seqs; b += 32) all += __shfl_sync(0xFFFFFFFFu, inclusive(units_of(b + lane)), 31);
-    int64_t units = units_of(lane), upto = inclusive(units);
-    all += __shfl_sync(0xFFFFFFFFu, upto, 31);
-    if (all < 1 || all > INT32_MAX) return;  // so many only from starts that overlap: the host refuses as much work
-    const int total = (int)all, ctas = min((int)gridDim.x, (total - 1) / (kLeastUnits + kSegment) + 1);
-    if (blockIdx.x >= ctas) return;
-    const Cut cut = {total / ctas, total % ctas};
-    const int from = cut.from(blockIdx.x), to = cut.from(blockIdx.x + 1);
-    for (int b = 0;;) {
-        const uint32_t here = __ballot_sync(0xFFFFFFFFu, upto - units <= from && from < upto);
-        if (here || b + 32 >= a.n_seqs) {  // the lane that has this CTA's first unit tells the others
-            const int src = here ? __ffs(here) - 1 : 0, rest = from - (int)__shfl_sync(0xFFFFFFFFu, upto - units, src);
-            place.s.first = __shfl_sync(0xFFFFFFFFu, place.s.first, src);
-            place.s.count = __shfl_sync(0xFFFFFFFFu, place.s.count, src);
-            place.s.len = __shfl_sync(0xFFFFFFFFu, place.s.len, src);
-            place.qtiles = __shfl_sync(0xFFFFFFFFu, place.qtiles, src);
-            place.tiles = __shfl_sync(0xFFFFFFFFu, place.tiles, src);
-            place.seq = b + src;
-            const int segment = rest / (place.tiles + kSegment);
-            place.tile = rest - segment * (place.tiles + kSegment);
-            place.head = segment / place.qtiles;
-            place.qtile = segment - place.head * place.qtiles;
-            break;
-        }
-        b += 32;
-        const int64_t before = __shfl_sync(0xFFFFFFFFu, upto, 31);
-        units = units_of(b + lane);
-        upto = before + inclusive(units);
-    }
-    int at_unit = from;  // place in the cut
-    if (place.tile >= place.tiles) {  // behind the segment's last unit: on to the next one
-        at_unit += place.tiles + kSegment - place.tile;
-        if (at_unit >= to) return;
-        next_segment<kRows>(a, place);
-    }
+    Part<kRows, kUnit, kSegment> part;
+    if (!part.find(a, gridDim.x, kLeastUnits)) return;
+    Place place = part.place;
+    const Cut cut = part.cut;
+    int at_unit = part.from;  // place in the cut
+    const int to = part.to;
     QueryBlocks<DIM, PARTS, NB, WARPS> raw;
     raw.load(a, place);
 
@@ -555,7 +430,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t v = head_word(head_at + (kUnit + 16 * h + 8 * e) * S::kHeads * 4);
                     value_step[h][e] = __uint_as_float(v & 0xFFFF0000u);
-                    size[h][e] = fmaxf(__uint_as_float(0x4B400000u + (v >> 23 & 255u)) - (kExactly + 127.0f), (float)kLeastSize);
+                    size[h][e] = size_of(v);
                 }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
@@ -682,7 +557,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
         if (done.tile + n == done.tiles) at_unit += kSegment;
         const bool more = at_unit < to;
         if (more) {  // the next segment's queries and first units, on their way meanwhile
-            next_segment<kRows>(a, place);
+            next_segment<kRows, kUnit>(a, place);
             raw.load(a, place);
             n = min(place.tiles, to - at_unit);
             my_units = begin(n);
@@ -733,7 +608,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
             }
             if (whole) {
                 const float part_of = highest == kNothing ? 0.0f : 1.0f / sum;
-                put_pair<PARTS, DIM>(a, done, kRows, r, d, v.x * part_of, v.y * part_of);
+                put_pair<PARTS == 2, DIM>(a, done, kRows, r, d, v.x * part_of, v.y * part_of);
                 if (d == 0) put_lse(a, done, kRows, r, highest, sum);
             } else {
                 *reinterpret_cast<float2*>(partial + 2 * kRows + r * DIM + d) = v;
@@ -745,95 +620,32 @@ k_cache_attend(const __grid_constant__ Attend a) {
         }
         __syncthreads();  // joined, and the parts written
         if (!whole) {  // the parts are those of the CTA with the segment's first unit to the one with its last
-            if (threadIdx.x == 0) {
-                const int first = at_unit - (done.tile + done_units == done.tiles ? kSegment : 0) - done_units - done.tile;
-                Pending& own = pending[n_pending];
-                own.place = done;
-                own.first_cta = cut.cta_of(first);
-                own.parts = cut.cta_of(first + done.tiles - 1) - own.first_cta + 1;
-                uint32_t before;
-                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + own.first_cta) : "memory");
-                arrived[n_pending] = before;  // looked at in the end: the answer takes its time
-            }
+            if (threadIdx.x == 0)
+                arrived[n_pending] = count_part(a, pending[n_pending], done, cut, at_unit - (done.tile + done_units == done.tiles ? kSegment : 0) - done_units - done.tile);
             ++n_pending;
         }
         if (!more) break;
         buffer ^= 1;
     }
 
-    // ---- the CTAs' parts into one, by the last CTA that has one, in the order of the CTAs
-    if (n_pending > 0) {
-        if (threadIdx.x == 0) {
-            for (int i = 0; i < n_pending; ++i) {
-                pending[i].is_last = arrived[i] == (uint32_t)(pending[i].parts - 1);
-                if (pending[i].is_last) a.counters[pending[i].first_cta] = 0;
-            }
-        }
-        __syncthreads();
-#pragma unroll 1
-        for (int i = 0; i < n_pending; ++i) {
-            if (!pending[i].is_last) continue;
-            const Place& done = pending[i].place;
-            const int rows = min(kRows, done.s.count * a.group - done.qtile * kRows), first_cta = pending[i].first_cta, parts = pending[i].parts;
-#pragma unroll 1
-            for (int at = threadIdx.x; at < rows * (DIM / 4); at += kThreads) {
-                const int r = at / (DIM / 4), d = at % (DIM / 4) * 4;
-                float highest = kNothing, sum = 0.0f;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                constexpr int kAtOnce = 8;
-#pragma unroll 1
-                for (int i0 = 0; i0 < parts; i0 += kAtOnce) {
-                    float m_of[kAtOnce], l_of[kAtOnce];
-                    float4 x[kAtOnce];
-#pragma unroll
-                    for (int k = 0; k < kAtOnce; ++k) {
-                        const float* part = a.partials + ((int64_t)(first_cta + i0 + k) * 2 + (i0 + k == 0 ? 1 : 0)) * kPart;
-                        m_of[k] = kNothing;
-                        if (i0 + k < parts) {
-                            m_of[k] = __ldcg(part + r);
-                            l_of[k] = __ldcg(part + kRows + r);
-                            x[k] = __ldcg(reinterpret_cast<const float4*>(part + 2 * kRows + r * DIM + d));
-                        }
-                    }
-                    float higher = highest;
-#pragma unroll
-                    for (int k = 0; k < kAtOnce; ++k) higher = larger(higher, m_of[k]);
-                    const float before = exp2_of(highest - higher);
-                    v.x *= before; v.y *= before; v.z *= before; v.w *= before;
-                    sum *= before;
-                    highest = higher;
-#pragma unroll
-                    for (int k = 0; k < kAtOnce; ++k) {
-                        const float keep = i0 + k < parts ? exp2_of(m_of[k] - highest) : 0.0f;
-                        if (keep != 0.0f) {
-                            v.x += x[k].x * keep; v.y += x[k].y * keep; v.z += x[k].z * keep; v.w += x[k].w * keep;
-                            sum += l_of[k] * keep;
-                        }
-                    }
-                }
-                const float part_of = highest == kNothing ? 0.0f : 1.0f / sum;
-                put_pair<PARTS, DIM>(a, done, kRows, r, d, v.x * part_of, v.y * part_of);
-                put_pair<PARTS, DIM>(a, done, kRows, r, d + 2, v.z * part_of, v.w * part_of);
-                if (d == 0) put_lse(a, done, kRows, r, highest, sum);
-            }
-        }
-    }
+    if (n_pending > 0) join_ctas<PARTS == 2, DIM, kRows>(a, pending, n_pending, arrived, kThreads);
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-constexpr int kMostRows = 16;
-int64_t scratch_bytes_of(int head_dim) { return 4 * kMostCtas + (int64_t)kMostCtas * 2 * kMostRows * (head_dim + 2) * 4; }
 
 template <int DIM, int PARTS, int NB, int WARPS, int CTAS>
 int launch_as(const Attend& a, cudaStream_t st) {
     using L = Layout<DIM, PARTS, NB, WARPS>;
     static_assert(CTAS * (L::kBytes + 1024) <= 228 * 1024, "shared memory");
-    static_assert(8 * NB <= kMostRows, "scratch memory");
+    static_assert(8 * NB <= kFewRows, "scratch memory");
     const auto kernel = k_cache_attend<DIM, PARTS, NB, WARPS, CTAS>;
     if (int e = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes), "cudaFuncSetAttribute")) return e;
     const int most = CTAS * sm_count(), grid = most < kMostCtas ? most : kMostCtas;
     return launch_dependent("e8_cache_attention", kernel, (unsigned)grid, 32 * WARPS, L::kBytes, st, a);
 }
+
+// Rows of a cache head, on average over the sequences, from which bf16 queries go to the kernel for many.
+constexpr int kFewRowsAtMost = 32;
 
 template <int DIM, int PARTS>
 int launch(const Attend& a, cudaStream_t st) {
@@ -846,7 +658,11 @@ int launch(const Attend& a, cudaStream_t st) {
 
 extern "C" {
 
-int64_t coset_e8_cache_attention_scratch_bytes(int head_dim) { return known_dim(head_dim) ? scratch_bytes_of(head_dim) : 0; }
+int64_t coset_e8_cache_attention_scratch_bytes(int head_dim) {
+    if (!known_dim(head_dim)) return 0;
+    const int64_t few = (int64_t)kMostCtas * kFewRows, many = head_dim == 256 ? 0 : (int64_t)kManyCtas * kManyRows;
+    return 4 * kMostCtas + (few > many ? few : many) * 2 * (head_dim + 2) * 4;
+}
 
 int coset_e8_cache_attention(const void* q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int n_queries, int q_heads, const void* pages,
                              int64_t n_pages, int n_heads, int page_size, int head_dim, const int32_t* table, int64_t table_stride, int max_pages,
@@ -879,6 +695,7 @@ int coset_e8_cache_attention(const void* q, int dtype, int64_t q_token_stride, i
     a.partials = (float*)scratch + kMostCtas;
     cudaStream_t st = (cudaStream_t)stream;
     const int bf16 = dtype == COSET_DTYPE_BF16;
+    if (bf16 && head_dim != 256 && ((int64_t)n_queries + n_seqs - 1) / n_seqs * a.group > kFewRowsAtMost) return launch_many(a, head_dim, st);
     if (head_dim == 64) return bf16 ? launch<64, 2>(a, st) : launch<64, 3>(a, st);
     if (head_dim == 128) return bf16 ? launch<128, 2>(a, st) : launch<128, 3>(a, st);
     return bf16 ? launch<256, 2>(a, st) : launch<256, 3>(a, st);
