@@ -644,8 +644,10 @@ int launch_as(const Attend& a, cudaStream_t st) {
     return launch_dependent("e8_cache_attention", kernel, (unsigned)grid, 32 * WARPS, L::kBytes, st, a);
 }
 
-// Rows of a cache head, on average over the sequences, from which bf16 queries go to the kernel for many.
-constexpr int kFewRowsAtMost = 32;
+// Up to so many rows of a cache head, on average over the sequences, stay here; bf16 queries with more go to the kernel for many.  8 cache heads of 128, us here and
+// there: 8 sequences of 500 to 3000 tokens with 16, 24, 32, 64 rows 27 and 28, 34 and 28, 37 and 29, 51 and 31; 4 of 8000 to 16384 with 16, 32, 64 rows 44 and
+// 55, 60 and 57, 97 and 60; 32 of 3000 to 6000 with 24 and 32 rows 129 and 147, 135 and 148.
+constexpr int kFewRowsAtMost = 24;
 
 template <int DIM, int PARTS>
 int launch(const Attend& a, cudaStream_t st) {
@@ -695,7 +697,8 @@ int coset_e8_cache_attention(const void* q, int dtype, int64_t q_token_stride, i
     a.partials = (float*)scratch + kMostCtas;
     cudaStream_t st = (cudaStream_t)stream;
     const int bf16 = dtype == COSET_DTYPE_BF16;
-    if (bf16 && head_dim != 256 && ((int64_t)n_queries + n_seqs - 1) / n_seqs * a.group > kFewRowsAtMost) return launch_many(a, head_dim, st);
+    const int64_t rows = ((int64_t)n_queries + n_seqs - 1) / n_seqs * a.group;  // of a cache head, on average over the sequences
+    if (bf16 && head_dim != 256 && rows > kFewRowsAtMost) return launch_many(a, head_dim, (int)rows, st);
     if (head_dim == 64) return bf16 ? launch<64, 2>(a, st) : launch<64, 3>(a, st);
     if (head_dim == 128) return bf16 ? launch<128, 2>(a, st) : launch<128, 3>(a, st);
     return bf16 ? launch<256, 2>(a, st) : launch<256, 3>(a, st);

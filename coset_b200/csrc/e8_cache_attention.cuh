@@ -59,7 +59,7 @@ constexpr float kNothing = -3.402823466e38f;  // running maximum of a row that h
 constexpr int kLeastSize = -90;   // exponent of a value's step as far as the running maximum goes: sums of p / 2^kLeastSize stay finite
 constexpr float kExactly = 12582912.0f;  // 1.5 2^23, see kExact
 // Scratch memory: a counter per CTA, zero between launches, and two parts per CTA of the rows of a tile: maxima, sums, results
-constexpr int kMostCtas = 304, kFewRows = 16, kManyRows = 128, kManyCtas = 152;
+constexpr int kMostCtas = 304, kFewRows = 16, kManyRows = 256, kManyCtas = 152;
 
 // The larger one; not a number where one of them is none.
 __device__ __forceinline__ float larger(float x, float y) {
@@ -277,7 +277,7 @@ __device__ __forceinline__ uint32_t count_part(const Attend& a, Pending& own, co
     return before;
 }
 
-int launch_many(const Attend& a, int head_dim, cudaStream_t stream);  // e8_cache_attention_many.cu
+int launch_many(const Attend& a, int head_dim, int rows, cudaStream_t stream);  // e8_cache_attention_many.cu
 
 }  // namespace cache
 }  // namespace coset
