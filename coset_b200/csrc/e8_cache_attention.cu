@@ -3,10 +3,11 @@
 //
 // Nothing dense is made.  A key is step (f + c / 2) with f + 8 a 4-bit number n, so
 //     q k / step = sum_i q_i n_i + sum_blocks c_b (sum of q over b) / 2 - 8 sum_i q_i,
-// and with q in fixed point (16 bits below the largest of a bf16 row, 24 of a float32 one, a power of two per row) all of it is a sum of products of
+// and with q in fixed point (24 bits from the row's largest on, a power of two per row) all of it is a sum of products of
 // bytes: three instructions make eight operands of a word of codes, the sums are exact in 32 bits, and start from the bits of 1.5 2^23, so that they are read
-// as floating-point numbers.  What a bf16 query loses is 2^-16 of its row's largest value, and nothing down to 2^-8 of it.  (As 8-bit floating-point
-// numbers, which a nibble is too, the products are no instruction of this chip but fourteen.)
+// as floating-point numbers.  What a query loses is 2^-24 of its row's largest value; bf16 loses nothing down to 2^-16 of it.  (Two bytes instead of three
+// take 5 % less time, but what they lose of small bf16 values shows in the logarithms of the sums: 1e-5.  As 8-bit floating-point numbers, which a nibble
+// is too, the products are no instruction of this chip but fourteen.)
 //     sum_j w_j v_j, w_j = p_j step_j, takes 16-bit products: a nibble under the exponent of 1024 (or 64, four bits up) less 1032 (72) is f.  (As the
 // subnormal number that its bits are it would need no subtraction, but the tensor cores line up products by their exponents and drop ten bits of such a
 // sum: results 1e-3 off.  Without the subtraction the sums' rounding, towards zero, counts 72 times: sum w f is small against sum w.)
@@ -33,6 +34,7 @@ namespace {
 
 constexpr int kUnit = 32;         // tokens of a warp's step
 constexpr int kLeastUnits = 4;    // of a CTA
+constexpr int kQueryBytes = 3;         // of a query in fixed point
 constexpr int kExact = 0x4B400000;  // the bits of kExactly = 1.5 2^23; a whole number of up to 22 bits added to them is added to it
 // What a segment costs a CTA beyond its units, in units: its queries, its first loads' latency, its joining.  The cut counts it.
 constexpr int kSegment = 16;
@@ -119,11 +121,11 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
 }
 
 // A tile of queries of one head in shared memory, in the order of the operands.  Part 0 of a number is its top byte, with the sign.
-template <int DIM, int PARTS, int NB>
+template <int DIM, int NB>
 struct Queries {
-    uint2 words[NB][DIM / 32][32][PARTS];                 // of word w: values 0, 2, 4, 6 and 1, 3, 5, 7 of its block
-    uint2 blocks[NB][PARTS][Shape<DIM>::kBitTiles][32];   // half the sums of four blocks: the part's bytes, and 64ths of what the top part is too small for
-    int start[PARTS][8 * NB];                             // kExact - 8 sum of the part
+    uint2 words[NB][DIM / 32][32][kQueryBytes];                 // of word w: values 0, 2, 4, 6 and 1, 3, 5, 7 of its block
+    uint2 blocks[NB][kQueryBytes][Shape<DIM>::kBitTiles][32];   // half the sums of four blocks: the part's bytes, and 64ths of what the top part is too small for
+    int start[kQueryBytes][8 * NB];                             // kExact - 8 sum of the part
     float factor[8 * NB];                                 // from a sum to a score in powers of two, but for the key's step
     uint64_t bits[8 * NB];                                // the queried tokens that a query sees
 };
@@ -137,20 +139,21 @@ struct Joining {
     static __device__ __forceinline__ int at(int d) { return d + 2 * (d / 16); }
 };
 
-template <int DIM, int PARTS, int NB, int WARPS>
+template <int DIM, int NB, int WARPS>
 struct Layout {
     static constexpr int kStages = DIM == 256 ? 2 : 3;
     static constexpr int kQueries = WARPS * kStages * Shape<DIM>::kStage;
-    static constexpr int kJoining = kQueries + 2 * (int)sizeof(Queries<DIM, PARTS, NB>);
+    static constexpr int kJoining = kQueries + 2 * (int)sizeof(Queries<DIM, NB>);
     static constexpr int kPending = kJoining + (int)sizeof(Joining<DIM, NB, WARPS>);
     static constexpr int kBytes = kPending + 2 * (int)sizeof(Pending);
 };
 
 // A thread's part of a tile of queries on its way to shared memory: blocks of 8 values of rows, whole warps at a time.
-template <int DIM, int PARTS, int NB, int WARPS>
+template <int DIM, bool BF16, int NB, int WARPS>
 struct QueryBlocks {
+    static constexpr int kQuads = BF16 ? 1 : 2;  // 16-byte words of a block
     static constexpr int kBlocks = DIM / 8, kAll = 8 * NB * kBlocks, kRounds = (kAll + 32 * WARPS - 1) / (32 * WARPS);
-    uint4 x[kRounds][PARTS - 1];
+    uint4 x[kRounds][kQuads];
     uint64_t bits[kRounds];
     __device__ __forceinline__ void load(const Attend& a, const Place& p) {
         const int rows = min(8 * NB, p.s.count * a.group - p.qtile * 8 * NB);
@@ -158,37 +161,37 @@ struct QueryBlocks {
         for (int i = 0; i < kRounds; ++i) {
             const int at = threadIdx.x + i * 32 * WARPS, r = at / kBlocks, b = at % kBlocks;
 #pragma unroll
-            for (int k = 0; k < PARTS - 1; ++k) x[i][k] = make_uint4(0, 0, 0, 0);
+            for (int k = 0; k < kQuads; ++k) x[i][k] = make_uint4(0, 0, 0, 0);
             bits[i] = 0;
             if (r < rows) {
                 const int row = p.qtile * 8 * NB + r, query = row / a.group;
                 const int64_t e = (p.s.first + query) * a.q_token_stride + (p.head * a.group + row - query * a.group) * a.q_head_stride + 8 * b;
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + e * (PARTS == 2 ? 2 : 4));
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + e * (BF16 ? 2 : 4));
 #pragma unroll
-                for (int k = 0; k < PARTS - 1; ++k) x[i][k] = __ldg(src + k);
+                for (int k = 0; k < kQuads; ++k) x[i][k] = __ldg(src + k);
                 if (b == 0) bits[i] = a.tree ? (uint64_t)__ldg(a.tree + p.s.first + query) : (uint64_t)query;
             }
         }
     }
-    __device__ __forceinline__ void put(const Attend& a, Queries<DIM, PARTS, NB>& s) const {
+    __device__ __forceinline__ void put(const Attend& a, Queries<DIM, NB>& s) const {
 #pragma unroll
         for (int i = 0; i < kRounds; ++i) {
             if (threadIdx.x / 32 * 32 + i * 32 * WARPS < kAll) put_one(a, s, threadIdx.x + i * 32 * WARPS, x[i], bits[i]);
         }
     }
-    static __device__ __forceinline__ void put_one(const Attend& a, Queries<DIM, PARTS, NB>& s, int at, const uint4 (&raw)[PARTS - 1], uint64_t bits) {
+    static __device__ __forceinline__ void put_one(const Attend& a, Queries<DIM, NB>& s, int at, const uint4 (&raw)[kQuads], uint64_t bits) {
         const int r = at / kBlocks, b = at % kBlocks;
         float x[8];
-        const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[PARTS - 2].x, raw[PARTS - 2].y, raw[PARTS - 2].z, raw[PARTS - 2].w};
+        const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[kQuads - 1].x, raw[kQuads - 1].y, raw[kQuads - 1].z, raw[kQuads - 1].w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = PARTS == 3 ? __uint_as_float(w[i]) : __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(!BF16 ? w[i] : i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
         uint32_t most = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);
 #pragma unroll
         for (int m = 1; m < kBlocks; m *= 2) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, m));
-        // fixed point: a power of two brings the row's largest into [2^(8 PARTS - 2), 2^(8 PARTS - 1))
-        constexpr int kTop = 8 * PARTS - 1;
+        // fixed point: a power of two brings the row's largest into [2^(8 kQueryBytes - 2), 2^(8 kQueryBytes - 1))
+        constexpr int kTop = 8 * kQueryBytes - 1;
         const bool number = most < 0x7F800000u;
         const int exponent = number ? min(kTop - 1 - ((int)(most >> 23) - 127), 126) : 0;
         const float up = number ? __uint_as_float((uint32_t)(exponent + 127) << 23) : 0.0f;
@@ -196,10 +199,10 @@ struct QueryBlocks {
 #pragma unroll
         for (int i = 0; i < 8; ++i) q[i] = number ? (uint32_t)min(__float2int_rn(x[i] * up), (1 << kTop) - 1) : 0u;
         const int lane = (r % 8) * 4 + b / (DIM / 32), word = b % (DIM / 32);
-        int part_sum[PARTS], sum = 0;
+        int part_sum[kQueryBytes], sum = 0;
 #pragma unroll
-        for (int j = 0; j < PARTS; ++j) {
-            const int byte = PARTS - 1 - j;  // of q
+        for (int j = 0; j < kQueryBytes; ++j) {
+            const int byte = kQueryBytes - 1 - j;  // of q
             const uint32_t pick = byte * 0x11 + 0x40;
             const uint32_t even = __byte_perm(__byte_perm(q[0], q[2], pick), __byte_perm(q[4], q[6], pick), 0x5410);
             const uint32_t odd = __byte_perm(__byte_perm(q[1], q[3], pick), __byte_perm(q[5], q[7], pick), 0x5410);
@@ -210,24 +213,24 @@ struct QueryBlocks {
         // bytes of half the block's sum, four blocks to a word
         const int half = (sum + 1) >> 1;
 #pragma unroll
-        for (int j = 0; j < PARTS; ++j) {
-            const int part = half >> (8 * (PARTS - 1 - j));
+        for (int j = 0; j < kQueryBytes; ++j) {
+            const int part = half >> (8 * (kQueryBytes - 1 - j));
             uint8_t* at_block = reinterpret_cast<uint8_t*>(&s.blocks[r / 8][j][word / 4][lane]) + (word & 3);
             at_block[0] = (uint8_t)(j == 0 ? part & 63 : part);
             at_block[4] = (uint8_t)(j == 0 ? part >> 6 : 0);
             if (DIM == 64) at_block[2] = at_block[6] = 0;  // a lane has two blocks of 64 values
         }
-        int total = part_sum[0] * 65536 + part_sum[PARTS - 1];  // both fit 16 bits when summed: |q| < 2^7 and 2^8 in 256 values
-        int middle = PARTS == 3 ? part_sum[1] : 0;
+        int total = part_sum[0] * 65536 + part_sum[kQueryBytes - 1];  // both fit 16 bits when summed: |q| < 2^7 and 2^8 in 256 values
+        int middle = part_sum[1];
 #pragma unroll
         for (int m = 1; m < kBlocks; m *= 2) {
             total += __shfl_xor_sync(0xFFFFFFFFu, total, m);
-            if (PARTS == 3) middle += __shfl_xor_sync(0xFFFFFFFFu, middle, m);
+            middle += __shfl_xor_sync(0xFFFFFFFFu, middle, m);
         }
         if (b == 0) {
-            s.start[PARTS - 1][r] = kExact - 8 * (total & 0xFFFF);
+            s.start[kQueryBytes - 1][r] = kExact - 8 * (total & 0xFFFF);
             s.start[0][r] = kExact - 8 * (total >> 16);
-            if (PARTS == 3) s.start[1][r] = kExact - 8 * middle;
+            s.start[1][r] = kExact - 8 * middle;
             s.factor[r] = number ? a.scale * 1.44269504f * __uint_as_float((uint32_t)(127 - exponent) << 23) : __uint_as_float(0x7FC00000u);
             s.bits[r] = bits;
         }
@@ -237,16 +240,16 @@ struct QueryBlocks {
 // Half a block's bit, from the sum over what the bit stands for as a 16-bit number
 template <int DIM>
 __device__ __forceinline__ float half_of_bit(int block) { return 0.5f / of_bit(block % (DIM / 64)); }
-template <int DIM, int PARTS, int NB, int WARPS, int CTAS>
+template <int DIM, bool BF16, int NB, int WARPS, int CTAS>
 __global__ void __launch_bounds__(32 * WARPS, CTAS)
 k_cache_attend(const __grid_constant__ Attend a) {
     using S = Shape<DIM>;
-    using L = Layout<DIM, PARTS, NB, WARPS>;
-    constexpr int kRows = 8 * NB, kThreads = 32 * WARPS, kWeights = PARTS - 1;  // 16-bit parts of a weight
+    using L = Layout<DIM, NB, WARPS>;
+    constexpr int kRows = 8 * NB, kThreads = 32 * WARPS, kWeights = BF16 ? 1 : 2;  // 16-bit parts of a weight
     constexpr int kPart = kRows * (DIM + 2);  // floats of a CTA's part: maxima, sums, rows; it has one for a segment that began before it and one for one that goes on behind it
-    constexpr float kSlack = PARTS == 3 ? 2.0f : 8.0f, kShift = PARTS == 3 ? 12.0f : 6.0f;  // weights reach 2^(1 + kSlack + kShift)
+    constexpr float kSlack = BF16 ? 8.0f : 2.0f, kShift = BF16 ? 6.0f : 12.0f;  // weights reach 2^(1 + kSlack + kShift)
     extern __shared__ __align__(128) uint8_t smem[];
-    auto* const all_queries = reinterpret_cast<Queries<DIM, PARTS, NB>*>(smem + L::kQueries);
+    auto* const all_queries = reinterpret_cast<Queries<DIM, NB>*>(smem + L::kQueries);
     auto& joining = *reinterpret_cast<Joining<DIM, NB, WARPS>*>(smem + L::kJoining);
     auto* const pending = reinterpret_cast<Pending*>(smem + L::kPending);
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -259,7 +262,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
     const Cut cut = part.cut;
     int at_unit = part.from;  // place in the cut
     const int to = part.to;
-    QueryBlocks<DIM, PARTS, NB, WARPS> raw;
+    QueryBlocks<DIM, BF16, NB, WARPS> raw;
     raw.load(a, place);
 
     // ---- fetching: the units of a segment's part, every WARPS-th for this warp.  Lane j knows where the rows of the j-th unit ahead are: the first and
@@ -361,9 +364,9 @@ k_cache_attend(const __grid_constant__ Attend a) {
             float s[2][NB][4], step[2][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                int sum[PARTS][NB][4];
+                int sum[kQueryBytes][NB][4];
 #pragma unroll
-                for (int j = 0; j < PARTS; ++j)
+                for (int j = 0; j < kQueryBytes; ++j)
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
                         const int2 s0 = *reinterpret_cast<const int2*>(&queries.start[j][8 * nb + 2 * t]);
@@ -386,15 +389,9 @@ k_cache_attend(const __grid_constant__ Attend a) {
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
                         const auto& q = queries.words[nb][w][lane];
-                        if (PARTS == 2) {
-                            const uint4 both = *reinterpret_cast<const uint4*>(&q[0]);
-                            mma_bytes<true>(sum[0][nb], x0, x1, x2, x3, both.x, both.y);
-                            mma_bytes<false>(sum[1][nb], x0, x1, x2, x3, both.z, both.w);
-                        } else {
-                            mma_bytes<true>(sum[0][nb], x0, x1, x2, x3, q[0].x, q[0].y);
+                        mma_bytes<true>(sum[0][nb], x0, x1, x2, x3, q[0].x, q[0].y);
 #pragma unroll
-                            for (int j = 1; j < PARTS; ++j) mma_bytes<false>(sum[j][nb], x0, x1, x2, x3, q[j].x, q[j].y);
-                        }
+                        for (int j = 1; j < kQueryBytes; ++j) mma_bytes<false>(sum[j][nb], x0, x1, x2, x3, q[j].x, q[j].y);
                     }
                 }
 #pragma unroll
@@ -404,7 +401,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                        for (int j = 0; j < PARTS; ++j) {
+                        for (int j = 0; j < kQueryBytes; ++j) {
                             const uint2 q = queries.blocks[nb][j][k][lane];
                             if (j == 0) mma_bytes<true>(sum[j][nb], x0, x1, x0 * 64, x1 * 64, q.x, q.y);
                             else mma_bytes<false>(sum[j][nb], x0, x1, x0, x1, q.x, 0);
@@ -416,7 +413,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
                     for (int i4 = 0; i4 < 4; ++i4) {
                         float x = __int_as_float(sum[0][nb][i4]) - kExactly;
 #pragma unroll
-                        for (int j = 1; j < PARTS; ++j) x = __fmaf_rn(x, 256.0f, __int_as_float(sum[j][nb][i4]) - kExactly);
+                        for (int j = 1; j < kQueryBytes; ++j) x = __fmaf_rn(x, 256.0f, __int_as_float(sum[j][nb][i4]) - kExactly);
                         s[h][nb][i4] = x;
                     }
             }
@@ -608,7 +605,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
             }
             if (whole) {
                 const float part_of = highest == kNothing ? 0.0f : 1.0f / sum;
-                put_pair<PARTS == 2, DIM>(a, done, kRows, r, d, v.x * part_of, v.y * part_of);
+                put_pair<BF16, DIM>(a, done, kRows, r, d, v.x * part_of, v.y * part_of);
                 if (d == 0) put_lse(a, done, kRows, r, highest, sum);
             } else {
                 *reinterpret_cast<float2*>(partial + 2 * kRows + r * DIM + d) = v;
@@ -628,32 +625,35 @@ k_cache_attend(const __grid_constant__ Attend a) {
         buffer ^= 1;
     }
 
-    if (n_pending > 0) join_ctas<PARTS == 2, DIM, kRows>(a, pending, n_pending, arrived, kThreads);
+    if (n_pending > 0) join_ctas<BF16, DIM, kRows>(a, pending, n_pending, arrived, kThreads);
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 
-template <int DIM, int PARTS, int NB, int WARPS, int CTAS>
+template <int DIM, bool BF16, int NB, int WARPS, int CTAS>
 int launch_as(const Attend& a, cudaStream_t st) {
-    using L = Layout<DIM, PARTS, NB, WARPS>;
+    using L = Layout<DIM, NB, WARPS>;
     static_assert(CTAS * (L::kBytes + 1024) <= 228 * 1024, "shared memory");
     static_assert(8 * NB <= kFewRows, "scratch memory");
-    const auto kernel = k_cache_attend<DIM, PARTS, NB, WARPS, CTAS>;
+    const auto kernel = k_cache_attend<DIM, BF16, NB, WARPS, CTAS>;
     if (int e = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes), "cudaFuncSetAttribute")) return e;
     const int most = CTAS * sm_count(), grid = most < kMostCtas ? most : kMostCtas;
     return launch_dependent("e8_cache_attention", kernel, (unsigned)grid, 32 * WARPS, L::kBytes, st, a);
 }
 
-// Up to so many rows of a cache head, on average over the sequences, stay here; bf16 queries with more go to the kernel for many.  8 cache heads of 128, us here and
-// there: 8 sequences of 500 to 3000 tokens with 16, 24, 32, 64 rows 27 and 28, 34 and 28, 37 and 29, 51 and 31; 4 of 8000 to 16384 with 16, 32, 64 rows 44 and
-// 55, 60 and 57, 97 and 60; 32 of 3000 to 6000 with 24 and 32 rows 129 and 147, 135 and 148.
-constexpr int kFewRowsAtMost = 24;
+// Up to so many rows of a cache head, on average over the sequences, stay here; bf16 queries with more go to the kernel for many.  8 cache heads, us here and
+// there: of 128 values, 8 sequences of 500 to 3000 tokens with 16, 24, 32 rows 26 and 27, 32 and 27, 36 and 28; 4 of 8000 to 16384 45 and 53, 61 and 53, 64 and
+// 55; 32 of 3000 to 6000 84 and 138, 146 and 139, 153 and 140; of 64 values, 8 of 500 to 3000 with 24, 32, 64 rows 22 and 24, 24 and 24, 35 and 25; 32 of 3000 to
+// 6000 with 24, 32 rows 97 and 114, 100 and 115.
+constexpr int few_rows_at_most(int head_dim) { return head_dim == 64 ? 32 : 16; }
 
-template <int DIM, int PARTS>
+template <int DIM, bool BF16>
 int launch(const Attend& a, cudaStream_t st) {
     const int64_t rows = ((int64_t)a.n_queries + a.n_seqs - 1) / a.n_seqs * a.group;  // of a cache head, on average
-    if (rows <= 8) return launch_as<DIM, PARTS, 1, DIM == 256 ? 6 : 4, DIM == 256 ? 1 : 2>(a, st);
-    return launch_as<DIM, PARTS, 2, DIM == 256 ? 4 : 4, DIM == 256 ? 1 : 2>(a, st);
+    // 256 values of 16 queries do not fit a thread's registers: 8 sequences of 500 to 3000 tokens with 16 rows 49 us in one tile, 36 in two of 8; 128 rows 166, 147
+    if constexpr (DIM == 256) return launch_as<DIM, BF16, 1, 6, 1>(a, st);
+    else if (rows <= 8) return launch_as<DIM, BF16, 1, 4, 2>(a, st);
+    else return launch_as<DIM, BF16, 2, 4, 2>(a, st);
 }
 
 }  // namespace
@@ -698,10 +698,10 @@ int coset_e8_cache_attention(const void* q, int dtype, int64_t q_token_stride, i
     cudaStream_t st = (cudaStream_t)stream;
     const int bf16 = dtype == COSET_DTYPE_BF16;
     const int64_t rows = ((int64_t)n_queries + n_seqs - 1) / n_seqs * a.group;  // of a cache head, on average over the sequences
-    if (bf16 && head_dim != 256 && rows > kFewRowsAtMost) return launch_many(a, head_dim, (int)rows, st);
-    if (head_dim == 64) return bf16 ? launch<64, 2>(a, st) : launch<64, 3>(a, st);
-    if (head_dim == 128) return bf16 ? launch<128, 2>(a, st) : launch<128, 3>(a, st);
-    return bf16 ? launch<256, 2>(a, st) : launch<256, 3>(a, st);
+    if (bf16 && head_dim != 256 && rows > few_rows_at_most(head_dim)) return launch_many(a, head_dim, (int)rows, st);
+    if (head_dim == 64) return bf16 ? launch<64, true>(a, st) : launch<64, false>(a, st);
+    if (head_dim == 128) return bf16 ? launch<128, true>(a, st) : launch<128, false>(a, st);
+    return bf16 ? launch<256, true>(a, st) : launch<256, false>(a, st);
 }
 
 }  // extern "C"
