@@ -313,6 +313,66 @@ def test_attention(shape, dtype, mask):
         assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])  # and the same bits every time
 
 
+MANY_ROWS = [
+    # rows of a cache head (group x queried tokens) around the sizes of tiles, lengths around theirs, segments that many CTAs share
+    (128, 1, 16, 16, [40], [1]),
+    (128, 1, 17, 16, [40], [1]),
+    (128, 1, 128, 16, [1], [1]),
+    (128, 2, 4, 16, [129, 128, 127], [5, 5, 5]),
+    (64, 1, 32, 32, [300], [1]),
+    (64, 1, 11, 32, [257], [3]),
+    (128, 1, 4, 64, [500, 37], [32, 32]),
+    (128, 1, 4, 64, [500, 37], [33, 33]),
+    (64, 2, 5, 1024, [1500], [51]),
+    (64, 1, 4, 16, [1000], [64]),
+    (128, 1, 6, 16, [900], [50]),
+    (64, 1, 8, 16, [2000], [64]),
+    (128, 1, 4, 128, [20000], [16]),
+    (128, 1, 8, 64, [9000, 9], [40, 40]),
+    (64, 2, 8, 64, [10000], [20]),
+]
+
+
+@pytest.mark.parametrize("mask", ["chain", "tree"])
+@pytest.mark.parametrize("shape", MANY_ROWS, ids=lambda s: f"d{s[0]}h{s[1]}g{s[2]}p{s[3]}n{max(s[4])}t{max(s[5])}")
+def test_attention_of_many_rows(shape, mask):
+    dim, heads, group, page, lens, counts = shape
+    pages, table = filled(dim, heads, page, lens, 17)
+    q = (rows(sum(counts), heads * group, dim, 22) * 1.5).to(torch.bfloat16).cuda()
+    check(q, pages, dim, table, lens, starts_of(counts), random_tree(counts, 5) if mask == "tree" else None)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim, group, lens, count", [(64, 2, [250, 190], 190), (128, 4, [300], 100), (256, 1, [140], 140)])
+def test_chains_longer_than_a_tree_can_be(dim, group, lens, count, dtype):
+    pages, table = filled(dim, 1, 16, lens, 18)
+    q = rows(count * len(lens), group, dim, 23, DTYPES[dtype]).cuda()
+    check(q, pages, dim, table, lens, starts_of([count] * len(lens)), None)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_rows_in_a_ragged_batch(dim):
+    """Sequences without queries, without tokens, with more queries than tokens, some of one tile and some of two; rows behind the last stay."""
+    lens, counts = [70, 0, 3, 400, 0, 129, 5], [64, 2, 9, 60, 0, 40, 1]
+    pages, table = filled(dim, 2, 32, lens, 4)
+    starts = starts_of(counts)
+    q = rows(starts[-1] + 4, 10, dim, 5, torch.bfloat16).cuda()
+    for tree in (None, random_tree(counts, 8) + [0] * 4):
+        out = torch.full_like(q, 5.0)
+        check(q, pages, dim, table, lens, starts, tree, out=out)
+        assert (out[starts[-1]:] == 5.0).all()
+
+
+@pytest.mark.parametrize("most", [2, 14])
+@pytest.mark.parametrize("n", [33, 70])
+def test_more_sequences_than_a_warp_has_lanes(n, most):
+    r = random.Random(n + most)
+    lens, counts = [r.randrange(0, 150) for _ in range(n)], [r.randrange(0, most + 1) for _ in range(n)]
+    pages, table = filled(128, 1, 16, lens, 6)
+    q = rows(sum(counts), 4, 128, 7, torch.bfloat16).cuda()
+    check(q, pages, 128, table, lens, starts_of(counts), None)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_ragged_batch_with_empty_sequences_and_rows_behind_the_last(dim, dtype):
@@ -340,7 +400,7 @@ def test_long_sequences_split_over_the_chip(tokens):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("tokens", [2, 40])
+@pytest.mark.parametrize("tokens", [2, 12, 40])
 def test_masked_places_hold_anything(tokens, dtype):
     """Infinities and NaN in tokens that a query does not see, and behind a sequence's end, leave its result alone; what it sees they reach."""
     kv = api()
@@ -367,8 +427,8 @@ def test_masked_places_hold_anything(tokens, dtype):
     assert torch.allclose(y[others].cpu().double(), want[0][others], rtol=2.0 ** -7, atol=2.0 ** -9) and torch.isfinite(y[others]).all()
 
 
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_values_of_very_different_sizes(dtype):
+@pytest.mark.parametrize("dtype, group", [("f32", 2), ("bf16", 2), ("bf16", 24), ("bf16", 72)])
+def test_values_of_very_different_sizes(dtype, group):
     """Values from 1e-30 to 1e30 in one sequence, rows of zeros, a huge value that one query does not see; scores that overflow exp."""
     kv = api()
     dim, page, L = 64, 16, 80
@@ -380,7 +440,7 @@ def test_values_of_very_different_sizes(dtype):
     v[-1] = 1e30
     k[5] *= 40
     kv.e8_cache_write(pages, k.cuda(), v.cuda(), slots)
-    q = (rows(2, 2, dim, 32) * 6).to(DTYPES[dtype]).cuda()
+    q = (rows(2, group, dim, 32) * 6).to(DTYPES[dtype]).cuda()
     check(q, pages, dim, table, [L], [0, 2], [1, 2])  # the first of two queried tokens does not see the last
     v[:] = 0
     kv.e8_cache_write(pages, k.cuda(), v.cuda(), slots)
@@ -392,11 +452,12 @@ def test_values_of_very_different_sizes(dtype):
         check(q, pages, dim, table, [L], [0, 2], None)
 
 
+@pytest.mark.parametrize("group", [2, 20])
 @pytest.mark.parametrize("size", [1e-30, 1e-4, 1.0, 300.0, 1e30])
-def test_queries_of_every_size(size):
+def test_queries_of_every_size(size, group):
     dim = 128
     pages, table = filled(dim, 1, 16, [50], 13)
-    q = rows(3, 2, dim, 14) * size
+    q = rows(3, group, dim, 14) * size
     q[0, 0, 5] = 50 * size
     q[1, 1] = 0
     for dtype in (torch.float32, torch.bfloat16):
@@ -507,13 +568,14 @@ def test_generation_step_by_step_in_a_graph():
         check(q, cache.pages, dim, table, now, list(range(B + 1)), None, got=results[i % 2])
 
 
-def test_two_streams_and_two_threads_at_once():
+@pytest.mark.parametrize("tokens", [1, 9, 40])
+def test_two_streams_and_two_threads_at_once(tokens):
     import threading
     kv = api()
     dim = 128
     pages, table = filled(dim, 2, 16, [900, 300], 5)
     t, n = torch.tensor(table, dtype=torch.int32, device="cuda"), torch.tensor([900, 300], dtype=torch.int32, device="cuda")
-    qs = [rows(2, 8, dim, s, torch.bfloat16).cuda() for s in range(4)]
+    qs = [rows(2 * tokens, 8, dim, s, torch.bfloat16).cuda() for s in range(4)]
     want = [kv.e8_cache_attention(q, pages, t, n) for q in qs]
     torch.cuda.synchronize()
     wrong = []
