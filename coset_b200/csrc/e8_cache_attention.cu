@@ -652,6 +652,10 @@ int launch(const Attend& a, cudaStream_t st) {
     const int64_t rows = ((int64_t)a.n_queries + a.n_seqs - 1) / a.n_seqs * a.group;  // of a cache head, on average
     // 256 values of 16 queries do not fit a thread's registers: 8 sequences of 500 to 3000 tokens with 16 rows 49 us in one tile, 36 in two of 8; 128 rows 166, 147
     if constexpr (DIM == 256) return launch_as<DIM, BF16, 1, 6, 1>(a, st);
+    // Fewer parts to join where few heads' tokens are shared by all CTAs, more overlap of one CTA's joining with the other's units elsewhere.  us with one CTA of 8
+    // warps and with two of 4: 8 heads of 131,071 tokens 49 and 55, of 32,000 19.7 and 20.5, 2 heads of 32,000 16.5 and 19.1; 64 of 4000 to 8000 24.2 and 22.8,
+    // 512 of 300 to 600 28.6 and 24.1.
+    else if (rows <= 8 && (int64_t)a.n_seqs * a.pages.n_heads < 16) return launch_as<DIM, BF16, 1, 8, 1>(a, st);
     else if (rows <= 8) return launch_as<DIM, BF16, 1, 4, 2>(a, st);
     else return launch_as<DIM, BF16, 2, 4, 2>(a, st);
 }
