@@ -70,38 +70,62 @@ struct Block<COSET_DTYPE_BF16> {
     }
 };
 
-// The code word of the nearest point to the scaled values x, and its bit c.  The bits of u + 1.5 2^23 hold u: its low 12, with their sign, are d, and bit 12 is
-// the last one of floor(u / 4096).  Of the sums of the floors and of f (the floor, and one more where d < 0) only the last bits are wanted, which
-// exclusive-or gives.
+// The larger (smaller) one of three
+__device__ __forceinline__ float largest(float x, float y, float z) {
+    float m;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+    return m;
+}
+__device__ __forceinline__ float smallest(float x, float y, float z) {
+    float m;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+    return m;
+}
+
+// The code word of the nearest point to the scaled values x, and its bit c.  All numbers are whole or have three bits behind the point, in float32 and two at
+// a time: u, f (halves up) and the floor h of u / 4096, d = u - 4096 f, and half words of four nibbles, sum 16^i (f + 8).  A number to be rounded is added to
+// 1.5 2^23, whose last bit then is the parity.  a goes with the place of its coordinate into one number, a + (7 - i) / 8 or a + i / 8.
 __device__ __forceinline__ uint32_t nearest_point(const float (&x)[8], float inv, bool* half) {
-    int u[8], d[8], top = 0, low = INT32_MAX, sum_a = 0;
-    uint32_t floors = 0, negative = 0;
+    const auto same = [](float v) { return two(v, v); };
+    float2 d[4];
+    Two f[4], h[4];
+    uint32_t odd_f = 0, odd_h = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // values i and i + 4
+        const Two u = add2(fma2(mul2(two(x[i], x[i + 4]), same(inv)), same(kGrid), same(kRound)), same(-kRound));  // the product with 4096 is exact
+        const Two to_f = fma2(add2(u, same(0.5f)), same(1.0f / kGrid), same(kRound)), to_h = fma2(add2(u, same(0.5f - kGrid / 2)), same(1.0f / kGrid), same(kRound));
+        f[i] = add2(to_f, same(-kRound));
+        h[i] = add2(to_h, same(-kRound));
+        d[i] = both(fma2(f[i], same(-kGrid), u));
+        odd_f ^= __float_as_uint(both(to_f).x) ^ __float_as_uint(both(to_f).y);
+        odd_h ^= __float_as_uint(both(to_h).x) ^ __float_as_uint(both(to_h).y);
+    }
+    float top[8], low[8], sum_a = kRound;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        u[i] = __float_as_int(__fmaf_rn(__fmul_rn(x[i], inv), kGrid, kRound));  // the product with 4096 is exact
-        d[i] = u[i] << 20 >> 20;
-        floors ^= (uint32_t)u[i];
-        negative ^= (uint32_t)d[i];
-        const int a = abs(d[i]);
+        const float a = fabsf(i < 4 ? d[i & 3].x : d[i & 3].y);
+        top[i] = a + (7 - i) * 0.125f;
+        low[i] = a + i * 0.125f;
         sum_a += a;
-        top = max(top, a * 8 + 7 - i);
-        low = min(low, a * 8 + i);
     }
-    const bool odd_h = floors >> 12 & 1, odd_f = (floors >> 12 ^ negative >> 31) & 1;
-    const int far = odd_f ? 4096 - 2 * (top >> 3) : 0, half_far = 8192 - sum_a + (odd_h ? 2 * (low >> 3) : 0);
+    const float topmost = largest(largest(largest(top[0], top[1], top[2]), top[3], top[4]), top[5], fmaxf(top[6], top[7]));
+    const float lowest = smallest(smallest(smallest(low[0], low[1], low[2]), low[3], low[4]), low[5], fminf(low[6], low[7]));
+    const int most = __float_as_int(__fmaf_rn(topmost, 8.0f, kRound)) - __float_as_int(kRound), least = __float_as_int(__fmaf_rn(lowest, 8.0f, kRound)) - __float_as_int(kRound);
+    odd_f &= 1;
+    odd_h &= 1;
+    const int far = odd_f ? 4096 - 2 * (most >> 3) : 0, half_far = 8192 - (__float_as_int(sum_a) - __float_as_int(kRound)) + (odd_h ? 2 * (least >> 3) : 0);
     const bool c = half_far < far;
-    const int offset = c ? 8 * 4096 : 8 * 4096 + 2048;  // to the nibble f + 8 at bits 12..15
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t y = (uint32_t)(u[i] + offset);
-        word |= (i < 3 ? y >> (12 - 4 * i) : y << (4 * i - 12)) & (15u << (4 * i));
-    }
+    const auto word_of = [&](const Two (&n)[4]) {
+        const float2 w = both(add2(fma2(fma2(fma2(n[3], same(16.0f), n[2]), same(16.0f), n[1]), same(16.0f), n[0]), same(8388608.0f + 0x8888)));
+        return __byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x5410);
+    };
+    const uint32_t word_f = word_of(f), word_h = word_of(h);
+    uint32_t word = c ? word_h : word_f;
     // the coordinate that moves: from the whole number towards the value, and from the half-odd one
-    const int k = c ? low & 7 : 7 - (top & 7);
-    const int d01 = k & 1 ? d[1] : d[0], d23 = k & 1 ? d[3] : d[2], d45 = k & 1 ? d[5] : d[4], d67 = k & 1 ? d[7] : d[6];
-    const int d03 = k & 2 ? d23 : d01, d47 = k & 2 ? d67 : d45, its = k & 4 ? d47 : d03;
-    const bool up = c ? its < 0 && its > -2048 : its > 0;
+    const int k = c ? least & 7 : 7 - (most & 7);
+    const float d04 = k & 4 ? d[0].y : d[0].x, d15 = k & 4 ? d[1].y : d[1].x, d26 = k & 4 ? d[2].y : d[2].x, d37 = k & 4 ? d[3].y : d[3].x;
+    const float even = k & 2 ? d26 : d04, odd = k & 2 ? d37 : d15, its = k & 1 ? odd : even;
+    const bool up = c ? its < 0.0f && its > -2048.0f : its > 0.0f;
     if (c ? odd_h : odd_f) word += (up ? 1u : 0xFFFFFFFFu) << (4 * k);
     *half = c;
     return word;

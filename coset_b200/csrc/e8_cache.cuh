@@ -33,6 +33,34 @@ struct Pages {
 template <int DIM>
 __device__ __forceinline__ int64_t record(const Pages& p, int64_t page, int head) { return ((page * p.n_heads + head) << p.page_log2) * row_words(DIM); }
 
+// Two float32 numbers at a time
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(float x, float y) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 both(Two x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ Two mul2(Two x, Two y) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ Two add2(Two x, Two y) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ Two fma2(Two x, Two y, Two z) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+
 inline bool known_dim(int dim) { return dim == 64 || dim == 128 || dim == 256; }
 
 // Checks of what every call is given; 0 or a negative status.

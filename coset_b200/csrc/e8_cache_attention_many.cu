@@ -82,34 +82,6 @@ __device__ __forceinline__ void umma_f16_from_tmem(uint32_t tmem_d, uint32_t tme
         ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// Two float32 numbers at a time
-using Two = unsigned long long;
-__device__ __forceinline__ Two two(float x, float y) {
-    Two r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ float2 both(Two x) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-    return r;
-}
-__device__ __forceinline__ Two mul2(Two x, Two y) {
-    Two r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return r;
-}
-__device__ __forceinline__ Two add2(Two x, Two y) {
-    Two r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return r;
-}
-__device__ __forceinline__ Two fma2(Two x, Two y, Two z) {
-    Two r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-    return r;
-}
-
 // Which of 32 tokens a query sees, the first of them `at` behind the first drafted one: as a chain (who: its place) or as a tree (who: its mask).
 __device__ __forceinline__ uint32_t seen_of(bool tree, uint64_t who, int at) {
     if (at <= -32) return 0xFFFFFFFFu;
