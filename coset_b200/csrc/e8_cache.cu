@@ -19,9 +19,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kRound = 12582912.0f;  // 1.5 2^23: added to a small number it rounds it to a whole one, which stands in the low 22 bits
 
-// A thread has a block of 8 values, DIM / 8 neighbours a row; a CTA has rows of one head, one token after the other, so that codes of tokens that
-// share a page are written and read as whole lines.  Rows of a CTA in one round:
-__host__ __device__ constexpr int rows_per_round(int dim) { return kThreads / (dim / 8); }
+// A thread has two blocks of 8 values, half a row apart (with one, finding the row costs as much as the search), DIM / 16 neighbours a row; a CTA has rows of
+// one head, one token after the other, so that codes of tokens that share a page are written and read as whole lines.  Rows of a CTA in one round:
+__host__ __device__ constexpr int rows_per_round(int dim) { return kThreads / (dim / 16); }
 
 template <int DT>
 struct Block;  // 8 values as they are in memory
@@ -148,48 +148,59 @@ struct Write {
 template <int DIM, int DT, int ROUNDS>
 __global__ void __launch_bounds__(kThreads)
 k_cache_write(const __grid_constant__ Write w) {
-    constexpr int kBlocks = DIM / 8, kRows = rows_per_round(DIM);
+    constexpr int kBlocks = DIM / 8, kLanes = DIM / 16, kRows = rows_per_round(DIM);
     grid_wait();
     grid_trigger();
-    const int b = threadIdx.x % kBlocks, lane = threadIdx.x & 31, which = blockIdx.y >= w.pages.n_heads, head = blockIdx.y - which * w.pages.n_heads;
-    const int64_t token0 = (int64_t)blockIdx.x * (kRows * ROUNDS) + threadIdx.x / kBlocks;
+    const int b = threadIdx.x % kLanes, lane = threadIdx.x & 31, which = blockIdx.y >= w.pages.n_heads, head = blockIdx.y - which * w.pages.n_heads;
+    const int64_t token0 = (int64_t)blockIdx.x * (kRows * ROUNDS) + threadIdx.x / kLanes;
     const void* x = (which ? w.x[1] : w.x[0]);
     const int64_t stride = which ? w.token_stride[1] : w.token_stride[0], first = head * (which ? w.head_stride[1] : w.head_stride[0]) + 8 * b;
     int64_t slot[ROUNDS];
-    Block<DT> raw[ROUNDS];
+    Block<DT> raw[ROUNDS][2];
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) slot[i] = token0 + i * kRows < w.n_tokens ? __ldg(behind_wait(w.slots) + token0 + i * kRows) : -1;
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
         if (slot[i] < 0 || slot[i] >> w.pages.page_log2 >= w.pages.n_pages) slot[i] = -1;
-        raw[i] = {};
-        if (slot[i] >= 0) raw[i].load(x, (token0 + i * kRows) * stride + first);
+        raw[i][0] = raw[i][1] = {};
+        if (slot[i] >= 0) {
+            const int64_t at = (token0 + i * kRows) * stride + first;
+            raw[i][0].load(x, at);
+            raw[i][1].load(x, at + DIM / 2);
+        }
     }
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
-        uint32_t most = raw[i].most();
+        uint32_t most = max(raw[i][0].most(), raw[i][1].most());
 #pragma unroll
-        for (int m = 1; m < kBlocks; m *= 2) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, m));
+        for (int m = 1; m < kLanes; m *= 2) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, m));
         const bool plain = most >= kSmallest && most < 0x7F800000u;
         uint32_t step = 0x3F800000u;
         if (plain) step = (__float_as_uint(seventh(__uint_as_float(most))) + 0xFFFFu) & 0xFFFF0000u;
-        float v[8];
-        raw[i].values(v);
-        if (!plain) {
+        const float inv = __frcp_rn(__uint_as_float(step));
+        uint32_t word[2], votes[2];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+        for (int j = 0; j < 2; ++j) {
+            float v[8];
+            raw[i][j].values(v);
+            if (!plain) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+            }
+            bool half;
+            word[j] = nearest_point(v, inv, &half);
+            votes[j] = __ballot_sync(0xFFFFFFFFu, half) >> (lane - b) & ((1u << kLanes) - 1u);
         }
-        bool half;
-        const uint32_t word = nearest_point(v, __frcp_rn(__uint_as_float(step)), &half);
-        const uint32_t votes = __ballot_sync(0xFFFFFFFFu, half);
         if (slot[i] < 0) continue;
         if (!plain) step = most < kSmallest ? 0u : kNoNumber;
         const int at = (int)slot[i] & ((1 << w.pages.page_log2) - 1);
         uint32_t* rec = w.pages.words + record<DIM>(w.pages, slot[i] >> w.pages.page_log2, head);
-        rec[((which << w.pages.page_log2) + at) * kBlocks + b] = word;
+        uint32_t* codes = rec + ((which << w.pages.page_log2) + at) * kBlocks + b;
+        codes[0] = word[0];
+        codes[kLanes] = word[1];
         if (b < head_words(DIM)) {
-            const uint32_t mine = votes >> (lane - b + 16 * b);
-            rec[((2 * kBlocks + which * head_words(DIM)) << w.pages.page_log2) + at * head_words(DIM) + b] = step | (mine & (kBlocks < 16 ? 0xFFu : 0xFFFFu));
+            const uint32_t bits = DIM == 256 ? (b ? votes[1] : votes[0]) : votes[0] | votes[1] << kLanes % 32;
+            rec[((2 * kBlocks + which * head_words(DIM)) << w.pages.page_log2) + at * head_words(DIM) + b] = step | bits;
         }
     }
 }
@@ -211,70 +222,79 @@ struct Read {
 template <int DIM, int DT, int ROUNDS>
 __global__ void __launch_bounds__(kThreads)
 k_cache_read(const __grid_constant__ Read r) {
-    constexpr int kBlocks = DIM / 8, kRows = rows_per_round(DIM);
+    constexpr int kBlocks = DIM / 8, kLanes = DIM / 16, kRows = rows_per_round(DIM);
     grid_wait();
     grid_trigger();
-    const int b = threadIdx.x % kBlocks, which = blockIdx.y >= r.pages.n_heads, head = blockIdx.y - which * r.pages.n_heads;
-    const int64_t token0 = (int64_t)blockIdx.x * (kRows * ROUNDS) + threadIdx.x / kBlocks;
+    const int b = threadIdx.x % kLanes, which = blockIdx.y >= r.pages.n_heads, head = blockIdx.y - which * r.pages.n_heads;
+    const int64_t token0 = (int64_t)blockIdx.x * (kRows * ROUNDS) + threadIdx.x / kLanes;
     int64_t slot[ROUNDS];
-    uint32_t word[ROUNDS], top[ROUNDS];
+    uint32_t word[ROUNDS][2], top[ROUNDS][2];
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) slot[i] = token0 + i * kRows < r.n_tokens ? __ldg(behind_wait(r.slots) + token0 + i * kRows) : -1;
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
-        word[i] = 0x88888888u;
-        top[i] = 0;
+        word[i][0] = word[i][1] = 0x88888888u;
+        top[i][0] = top[i][1] = 0;
         if (slot[i] >= 0 && slot[i] >> r.pages.page_log2 < r.pages.n_pages) {
             const int at = (int)slot[i] & ((1 << r.pages.page_log2) - 1);
             const uint32_t* rec = r.pages.words + record<DIM>(r.pages, slot[i] >> r.pages.page_log2, head);
-            word[i] = rec[((which << r.pages.page_log2) + at) * kBlocks + b];
-            top[i] = rec[((2 * kBlocks + which * head_words(DIM)) << r.pages.page_log2) + at * head_words(DIM) + b / 16];
+            const uint32_t* codes = rec + ((which << r.pages.page_log2) + at) * kBlocks + b;
+            word[i][0] = codes[0];
+            word[i][1] = codes[kLanes];
+            const uint32_t* heads = rec + ((2 * kBlocks + which * head_words(DIM)) << r.pages.page_log2) + at * head_words(DIM);
+            top[i][0] = heads[0];
+            top[i][1] = DIM == 256 ? heads[1] : top[i][0];
         }
     }
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
         if (token0 + i * kRows >= r.n_tokens) continue;
-        const int64_t to = ((token0 + i * kRows) * r.pages.n_heads + head) * DIM + 8 * b;
         void* out = which ? r.out[1] : r.out[0];
-        const uint32_t c = top[i] >> (b % 16) & 1;
-        if (DT == COSET_DTYPE_F32) {
-            // a nibble at bits 1..4 under the exponent of 2^22, and c at bit 0, is the number 2^22 + n + c / 2
-            const float step = __uint_as_float(top[i] & 0xFFFF0000u);
-            float v[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const uint32_t shifted = k == 0 ? word[i] << 1 : word[i] >> (4 * k - 1);
-                v[k] = __fmul_rn(__uint_as_float(chosen(shifted, 0x1Eu, 0x4A800000u | c)) - 4194312.0f, step);
-            }
-            float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + to);
-            __stcs(p, make_float4(v[0], v[1], v[2], v[3]));
-            __stcs(p + 1, make_float4(v[4], v[5], v[6], v[7]));
-        } else {
-            // the same in bf16, two at a time: 64 + n + c / 2, less 72; the product with the step is rounded once, as the float32 product would be
-            const uint32_t exponent = 0x42804280u | c * 0x00010001u, step = __byte_perm(top[i], 0, 0x3232);
-            uint32_t v[4];
+        for (int j = 0; j < 2; ++j) {
+            const int64_t to = ((token0 + i * kRows) * r.pages.n_heads + head) * DIM + 8 * b + j * (DIM / 2);
+            const uint32_t c = top[i][j] >> (DIM == 256 ? b : b + j * kLanes) & 1, its = word[i][j];
+            if (DT == COSET_DTYPE_F32) {
+                // a nibble at bits 1..4 under the exponent of 2^22, and c at bit 0, is the number 2^22 + n + c / 2
+                const float step = __uint_as_float(top[i][j] & 0xFFFF0000u);
+                float v[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {  // values k and k + 4
-                const uint32_t shifted = k == 0 ? word[i] << 1 : word[i] >> (4 * k - 1);
-                asm("{\n\t.reg .b32 t;\n\tadd.rn.bf16x2 t, %1, %2;\n\tmul.rn.bf16x2 %0, t, %3;\n\t}" : "=r"(v[k]) : "r"(chosen(shifted, 0x001E001Eu, exponent)), "r"(0xC290C290u), "r"(step));
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t shifted = k == 0 ? its << 1 : its >> (4 * k - 1);
+                    v[k] = __fmul_rn(__uint_as_float(chosen(shifted, 0x1Eu, 0x4A800000u | c)) - 4194312.0f, step);
+                }
+                float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + to);
+                __stcs(p, make_float4(v[0], v[1], v[2], v[3]));
+                __stcs(p + 1, make_float4(v[4], v[5], v[6], v[7]));
+            } else {
+                // the same in bf16, two at a time: 64 + n + c / 2, less 72; the product with the step is rounded once, as the float32 product would be
+                const uint32_t exponent = 0x42804280u | c * 0x00010001u, step = __byte_perm(top[i][j], 0, 0x3232);
+                uint32_t v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {  // values k and k + 4
+                    const uint32_t shifted = k == 0 ? its << 1 : its >> (4 * k - 1);
+                    asm("{\n\t.reg .b32 t;\n\tadd.rn.bf16x2 t, %1, %2;\n\tmul.rn.bf16x2 %0, t, %3;\n\t}" : "=r"(v[k]) : "r"(chosen(shifted, 0x001E001Eu, exponent)), "r"(0xC290C290u), "r"(step));
+                }
+                __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to),
+                       make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)));
             }
-            __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to),
-                   make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)));
         }
     }
 }
 
 bool known_dtype(int dtype) { return dtype == COSET_DTYPE_F32 || dtype == COSET_DTYPE_BF16; }
 
-// The grid of a call, and whether its CTAs do four rounds: from four CTAs per SM on.
+// The grid of a call, and whether its CTAs do two rounds: of bf16 tokens from four CTAs per SM on.  us with two rounds and with one, heads of 128: writing 8192
+// bf16 tokens of 8 heads 17.6 and 18.1, 32768 61.5 and 63.8, reading 32768 27.1 (96 % of the copy rate) and 28.2; writing 8192 float32 ones 18.8 and 19.7,
+// reading them 17.6 and 15.1.  Writes are bound by the issue of some 220 instructions per two blocks, reads by memory.
 struct Shape {
     dim3 grid;
-    bool many;
+    bool twice;
 };
-int shape_of(int64_t n_tokens, int n_heads, int dim, Shape* s) {
+int shape_of(int64_t n_tokens, int n_heads, int dim, int dtype, Shape* s) {
     const int64_t rows = rows_per_round(dim), once = (n_tokens + rows - 1) / rows;
-    s->many = once * 2 * n_heads >= 16 * (int64_t)sm_count();
-    const int64_t x = s->many ? (once + 3) / 4 : once;
+    s->twice = dtype == COSET_DTYPE_BF16 && once * 2 * n_heads >= 8 * (int64_t)sm_count();
+    const int64_t x = s->twice ? (once + 1) / 2 : once;
     if (x > INT32_MAX) return fail(COSET_E_UNSUPPORTED, "too many tokens for one call");
     s->grid = dim3((unsigned)x, 2 * (unsigned)n_heads);
     return 0;
@@ -282,13 +302,15 @@ int shape_of(int64_t n_tokens, int n_heads, int dim, Shape* s) {
 
 template <int DIM, int DT>
 int launch_write(const Write& w, const Shape& s, cudaStream_t st) {
-    return s.many ? launch_dependent("e8_cache_write", k_cache_write<DIM, DT, 4>, s.grid, kThreads, 0, st, w)
-                  : launch_dependent("e8_cache_write", k_cache_write<DIM, DT, 1>, s.grid, kThreads, 0, st, w);
+    if constexpr (DT == COSET_DTYPE_BF16)
+        if (s.twice) return launch_dependent("e8_cache_write", k_cache_write<DIM, DT, 2>, s.grid, kThreads, 0, st, w);
+    return launch_dependent("e8_cache_write", k_cache_write<DIM, DT, 1>, s.grid, kThreads, 0, st, w);
 }
 template <int DIM, int DT>
 int launch_read(const Read& r, const Shape& s, cudaStream_t st) {
-    return s.many ? launch_dependent("e8_cache_read", k_cache_read<DIM, DT, 4>, s.grid, kThreads, 0, st, r)
-                  : launch_dependent("e8_cache_read", k_cache_read<DIM, DT, 1>, s.grid, kThreads, 0, st, r);
+    if constexpr (DT == COSET_DTYPE_BF16)
+        if (s.twice) return launch_dependent("e8_cache_read", k_cache_read<DIM, DT, 2>, s.grid, kThreads, 0, st, r);
+    return launch_dependent("e8_cache_read", k_cache_read<DIM, DT, 1>, s.grid, kThreads, 0, st, r);
 }
 template <int DIM>
 int launch_write(const Write& w, int dtype, const Shape& s, cudaStream_t st) {
@@ -323,7 +345,7 @@ int coset_e8_cache_write(void* pages, int64_t n_pages, int n_heads, int page_siz
     w.slots = slots;
     w.n_tokens = n_tokens;
     Shape shape;
-    if (int e = shape_of(n_tokens, n_heads, head_dim, &shape)) return e;
+    if (int e = shape_of(n_tokens, n_heads, head_dim, dtype, &shape)) return e;
     cudaStream_t st = (cudaStream_t)stream;
     return head_dim == 64 ? launch_write<64>(w, dtype, shape, st) : head_dim == 128 ? launch_write<128>(w, dtype, shape, st) : launch_write<256>(w, dtype, shape, st);
 }
@@ -341,7 +363,7 @@ int coset_e8_cache_read(const void* pages, int64_t n_pages, int n_heads, int pag
     r.slots = slots;
     r.n_tokens = n_tokens;
     Shape shape;
-    if (int e = shape_of(n_tokens, n_heads, head_dim, &shape)) return e;
+    if (int e = shape_of(n_tokens, n_heads, head_dim, dtype, &shape)) return e;
     cudaStream_t st = (cudaStream_t)stream;
     return head_dim == 64 ? launch_read<64>(r, dtype, shape, st) : head_dim == 128 ? launch_read<128>(r, dtype, shape, st) : launch_read<256>(r, dtype, shape, st);
 }
