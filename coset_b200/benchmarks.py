@@ -3,6 +3,7 @@ exist, pyproject.toml:67).  One JSON line per measurement:
 
     python -m coset_b200.benchmarks qat        # E8HNLQLinear QAT step, W [3072, 768], 4096 bf16 tokens
     python -m coset_b200.benchmarks vlut       # code-domain matmul, W [4096, 4096], T in {1, 16, 256, 4096}
+    python -m coset_b200.benchmarks kvcache    # E8-coded key/value cache: writes, reads, attention; 8 heads of 128
     python -m torch.distributed.run --nproc-per-node N -m coset_b200.benchmarks gradcomm
                                                # E8-quantised gradient exchange, BERT-base-shaped gradient
     python -m coset_b200.benchmarks profile-gemv | profile-gemv16 | profile-gemm | profile-gemm-pair | profile-dense | profile-f32
@@ -241,6 +242,39 @@ def bench_d4():
                           "peaks": src}), flush=True)
 
 
+def iter_kvcache():
+    """The E8-coded cache of a model with 8 key/value heads of 128 and 32 query heads: writes, reads, and attention of one token and of trees of
+    drafted tokens per sequence."""
+    from . import kvcache
+    hbm, _, src = peaks()
+    heads, group, dim, page = 8, 4, 128, 64
+    for n in (32, 8192):
+        pages = kvcache.e8_cache_pages(n // page + 1, heads, page, dim)
+        k = torch.randn(n, heads, dim, device="cuda").bfloat16()
+        slots = torch.randperm(n, device="cuda")
+        by = n * heads * 2 * (2 * dim + dim // 2 + 4)
+        for name, fn in (("write", lambda: kvcache.e8_cache_write(pages, k, k, slots)), ("read", lambda: kvcache.e8_cache_read(pages, slots, torch.bfloat16))):
+            ms = cuda_time(fn)
+            yield {"bench": f"kvcache_{name}", "tokens": n, "ms": ms, "GBps": by / (ms * 1e-3) / 1e9, "frac_of_hbm": by / (ms * 1e-3) / 1e9 / hbm, "peaks": src}
+    for seqs, length, tokens in ((1, 1000, 1), (32, 6000, 1), (1, 131072, 1), (8, 2000, 8), (4, 12000, 64)):
+        per = (length + page - 1) // page
+        pages = kvcache.e8_cache_pages(seqs * per, heads, page, dim)
+        k = torch.randn(seqs * per * page, heads, dim, device="cuda").bfloat16()
+        kvcache.e8_cache_write(pages, k, k, torch.arange(seqs * per * page, device="cuda"))
+        table = torch.randperm(seqs * per, device="cuda").int().view(seqs, per)
+        lens = torch.full((seqs,), length, dtype=torch.int32, device="cuda")
+        q = torch.randn(seqs * tokens, heads * group, dim, device="cuda").bfloat16()
+        ms = cuda_time(lambda: kvcache.e8_cache_attention(q, pages, table, lens))
+        by = seqs * length * heads * 2 * (dim // 2 + 4)
+        yield {"bench": "kvcache_attention", "seqs": seqs, "length": length, "queried_tokens": tokens, "ms": ms, "GBps": by / (ms * 1e-3) / 1e9,
+               "frac_of_hbm": by / (ms * 1e-3) / 1e9 / hbm, "dense_bytes_per_code_byte": 4 * dim / (dim + 8), "peaks": src}
+
+
+def bench_kvcache():
+    for rec in iter_kvcache():
+        print(json.dumps(rec), flush=True)
+
+
 def bench_vlut_sharded():
     """Config-4 weight split along the output features over the ranks of a torchrun launch: every
     rank multiplies its [4096 / W, 4096] slice, one all-gather of the outputs follows."""
@@ -392,6 +426,8 @@ def main(argv=None):
         bench_vlut()
     if which in ("d4", "all"):
         bench_d4()
+    if which in ("kvcache", "all"):
+        bench_kvcache()
     if which == "vlut_sharded":
         bench_vlut_sharded()
     if which in ("gradcomm", "all"):

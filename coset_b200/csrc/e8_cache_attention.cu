@@ -667,7 +667,8 @@ extern "C" {
 int64_t coset_e8_cache_attention_scratch_bytes(int head_dim) {
     if (!known_dim(head_dim)) return 0;
     const int64_t few = (int64_t)kMostCtas * kFewRows, many = head_dim == 256 ? 0 : (int64_t)kManyCtas * kManyRows;
-    return 4 * kMostCtas + (few > many ? few : many) * 2 * (head_dim + 2) * 4;
+    static_assert(4 * kMostCtas <= COSET_E8_CACHE_SCRATCH_ZEROS, "the counters");
+    return COSET_E8_CACHE_SCRATCH_ZEROS + (few > many ? few : many) * 2 * (head_dim + 2) * 4;
 }
 
 int coset_e8_cache_attention(const void* q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int n_queries, int q_heads, const void* pages,
@@ -698,7 +699,7 @@ int coset_e8_cache_attention(const void* q, int dtype, int64_t q_token_stride, i
     a.table = table; a.table_stride = table_stride; a.max_pages = max_pages; a.lens = lens; a.starts = q_starts; a.n_seqs = n_seqs;
     a.tree = tree; a.scale = scale; a.out = out; a.lse = lse;
     a.counters = (uint32_t*)scratch;
-    a.partials = (float*)scratch + kMostCtas;
+    a.partials = (float*)scratch + COSET_E8_CACHE_SCRATCH_ZEROS / 4;
     cudaStream_t st = (cudaStream_t)stream;
     const int bf16 = dtype == COSET_DTYPE_BF16;
     const int64_t rows = ((int64_t)n_queries + n_seqs - 1) / n_seqs * a.group;  // of a cache head, on average over the sequences

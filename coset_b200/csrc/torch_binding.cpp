@@ -850,10 +850,14 @@ PyObject* cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// The attention's scratch: kept for each stream, whose calls follow one another.  A capture gets one of its own, cleared in the graph, so that a
-// replay shares it with no other call.
+// The attention's scratch: kept for each stream, whose calls follow one another.  A capture gets one of its own, its counters cleared in the graph, so that
+// a replay shares it with no other call.
 Tensor attention_scratch(int64_t bytes, const Tensor& like) {
-    const auto fresh = [&]() { return empty({bytes}, at::kByte, like).zero_(); };
+    const auto fresh = [&]() {
+        Tensor t = empty({bytes}, at::kByte, like);
+        t.narrow(0, 0, std::min<int64_t>(bytes, COSET_E8_CACHE_SCRATCH_ZEROS)).zero_();
+        return t;
+    };
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(like.get_device()).stream();
     if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return fresh();
     static std::mutex mutex;

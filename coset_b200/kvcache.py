@@ -71,7 +71,12 @@ def e8_cache_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor
     out: receives the result (contiguous, of q's shape, type and device, and not q's memory).  Rows of q behind the last sequence are left as
       they were in `out`, and hold anything in a result that is made here.
 
-    A query that sees nothing gives zeros (and -inf).  Sums are float32; float32 queries are multiplied as such."""
+    A query that sees nothing gives zeros (and -inf).  Queries count with 24 bits from the largest of their row on, sums and the softmax's statistics are
+    float32, and weights are rounded to 11 bits for bf16 queries, to 22 for float32 ones.  Where a tree's or a chain's queries of a cache head are
+    more than 16 (32 of 64 values) on average, bf16 products run on tcgen05 and sum in another order: results agree to the rounding, not to the bit.  Equal
+    calls give equal bits.
+
+    The call keeps a scratch buffer of 20 to 40 MB per device and stream (one per call that is captured into a graph)."""
     return _lib.native().cache_attention(q, pages, table, lens, q_starts, tree, 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale),
                                          bool(return_lse), out)
 

@@ -468,9 +468,12 @@ int coset_e8_cache_read(const void* pages, int64_t n_pages, int n_heads, int pag
  *   tree   : [n_queries] bit j: the query sees queried token j of its sequence (itself among them; tokens from 64 on are not seen).  null: a chain,
  *            every query sees the queried tokens up to itself.  All earlier tokens of the sequence are seen by all its queries.
  *   out    : [n_queries, q_heads, head_dim] of q's type;  lse: [n_queries, q_heads] float32, may be null
- * A query that sees nothing gives zeros and -infinity.  scratch: coset_e8_cache_attention_scratch_bytes(head_dim) bytes, 16-byte aligned, zero
- * before the first use and left so by every call; calls that may overlap on the device need one each.  One launch; sums are float32.
+ * A query that sees nothing gives zeros and -infinity.  scratch: coset_e8_cache_attention_scratch_bytes(head_dim) bytes, 16-byte aligned,
+ * the first COSET_E8_CACHE_SCRATCH_ZEROS of them zero before the first use and left so by every call; calls that may overlap on the device need one each.
+ * One launch; sums are float32.  Limits: n_heads up to 32767, fewer than 2^32 records, sequences below 2^31 tokens, and (queries / 8 + sequences) x
+ * heads x (max_pages * page_size / 32 + 17) up to 2e9.
  */
+#define COSET_E8_CACHE_SCRATCH_ZEROS 4096
 int64_t coset_e8_cache_attention_scratch_bytes(int head_dim);
 int coset_e8_cache_attention(const void* q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int n_queries, int q_heads, const void* pages,
                              int64_t n_pages, int n_heads, int page_size, int head_dim, const int32_t* table, int64_t table_stride, int max_pages,
