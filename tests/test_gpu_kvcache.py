@@ -464,13 +464,14 @@ def test_queries_of_every_size(size, group):
         check(q.to(dtype).cuda(), pages, dim, table, [50], [0, 3], None, scale=min(1.0, 1.0 / size) / math.sqrt(dim))
 
 
-def test_pages_outside_the_cache_are_not_seen():
+@pytest.mark.parametrize("group, dtype", [(1, "f32"), (24, "bf16"), (80, "bf16")])
+def test_pages_outside_the_cache_are_not_seen(group, dtype):
     kv = api()
     dim, page = 64, 16
     lens = [60, 40]
     pages, table = filled(dim, 2, page, lens, 5)
     table[0][1], table[1][0], table[1][1], table[1][2] = -1, pages.shape[0], 2 ** 31 - 1, -2 ** 31
-    q = rows(4, 2, dim, 6).cuda()
+    q = rows(4, 2 * group, dim, 6, DTYPES[dtype]).cuda()
     got = check(q, pages, dim, table, lens, [0, 2, 4], None)
     assert torch.equal(got[0][2:], torch.zeros_like(got[0][2:])) and (got[1][2:] == -math.inf).all()
     lens = [1000, 100]  # more than the table lists
@@ -484,14 +485,15 @@ def test_pages_outside_the_cache_are_not_seen():
     assert not y.any() and (z == -math.inf).all()
 
 
-def test_starts_that_make_no_sense_touch_nothing_outside():
+@pytest.mark.parametrize("heads, dtype", [(2, torch.float32), (24, torch.bfloat16), (80, torch.bfloat16)])
+def test_starts_that_make_no_sense_touch_nothing_outside(heads, dtype):
     """Starts that descend, lie outside, or overlap: every access stays inside, and a later call is right."""
     kv = api()
     pages, table = filled(64, 1, 16, [40, 40, 40], 5)
-    q = rows(6, 2, 64, 6).cuda()
+    q = rows(6, heads, 64, 6, dtype).cuda()
     t, n = torch.tensor(table, dtype=torch.int32, device="cuda"), torch.tensor([40] * 3, dtype=torch.int32, device="cuda")
     for starts in ([0, 4, 2, 6], [-5, 2, 100, 2 ** 31 - 1], [-2 ** 31, -1, -1, 3], [6, 6, 6, 6], [0, 2 ** 31 - 1, 0, 2 ** 31 - 1], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, -2 ** 31]):
-        guard = torch.full((18, 2, 64), 3.0, device="cuda")
+        guard = torch.full((18, heads, 64), 3.0, dtype=dtype, device="cuda")
         kv.e8_cache_attention(q, pages, t, n, q_starts=torch.tensor(starts, dtype=torch.int32, device="cuda"), out=guard[6:12])
         assert (guard[:6] == 3.0).all() and (guard[12:] == 3.0).all()
     check(q, pages, 64, table, [40] * 3, [0, 1, 3, 6], None)
@@ -566,6 +568,34 @@ def test_generation_step_by_step_in_a_graph():
         graphs[i % 2].replay()
         torch.cuda.synchronize()
         check(q, cache.pages, dim, table, now, list(range(B + 1)), None, got=results[i % 2])
+
+
+@pytest.mark.parametrize("tokens", [1, 9, 40])
+def test_two_captured_graphs_at_once(tokens):
+    """Two graphs of the same call replayed on two streams at the same time, with lengths that changed since, beside eager calls."""
+    kv = api()
+    dim = 128
+    pages, table = filled(dim, 2, 16, [900, 300], 5)
+    t = torch.tensor(table, dtype=torch.int32, device="cuda")
+    tree = signed(random_tree([tokens] * 2, 9))
+    lens = torch.tensor([100, 60], dtype=torch.int32, device="cuda")
+    q = rows(2 * tokens, 8, dim, 3, torch.bfloat16).cuda()
+    kv.e8_cache_attention(q, pages, t, lens, tree=tree)
+    streams, graphs, results = [torch.cuda.Stream() for _ in range(2)], [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            results.append(kv.e8_cache_attention(q, pages, t, lens, tree=tree))
+    for now in ([900, 300], [64, 64], [577, 1]):
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for s, g in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    g.replay()
+            want = kv.e8_cache_attention(q, pages, t, lens, tree=tree)
+        torch.cuda.synchronize()
+        assert torch.equal(results[0], want) and torch.equal(results[1], want)
 
 
 @pytest.mark.parametrize("tokens", [1, 9, 40])
