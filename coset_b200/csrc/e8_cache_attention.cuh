@@ -57,7 +57,7 @@ __device__ __forceinline__ int page_of(const Attend& a, int b, int token, int le
 
 constexpr float kNothing = -3.402823466e38f;  // running maximum of a row that has seen nothing
 constexpr int kLeastSize = -90;   // exponent of a value's step as far as the running maximum goes: sums of p / 2^kLeastSize stay finite
-constexpr float kExactly = 12582912.0f;  // 1.5 2^23, see kExact
+constexpr float kExactly = 12582912.0f;  // 1.5 2^23, to whose last bits small whole numbers are added
 // Scratch memory: a counter per CTA, zero between launches, and two parts per CTA of the rows of a tile: maxima, sums, results
 constexpr int kMostCtas = 304, kFewRows = 16, kManyRows = 256, kManyCtas = 152;
 

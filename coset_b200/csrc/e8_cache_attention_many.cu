@@ -17,6 +17,10 @@
 // shared memory's pipe 57 %, tensor cores 28 %): what bounds it is the softmax's chain of dependent instructions in two warps per scheduler.  Without any one
 // of decoding, maxima, weights, loads of steps it would be 3 to 15 % faster.  Tried: one group with halves of rows 232 us; eight decoding warps and registers
 // moved to the softmax 197; loops over tokens unrolled by two or with tensor memory's loads ahead 196 and 235, by 16 instead of 32 tokens 205.
+//
+// With up to 128 queries (32 sequences of 3000 to 6000 tokens, 32 rows: 140 us) a tile takes some 3800 cycles and the decoding warps bound it: keys and values 850 each with
+// the fence behind them, addresses and loads 1500, waits 700.  Two tiles' codes ahead in registers of eight warps 138 us, asynchronous copies to shared memory 137, their
+// loops not unrolled 152; the smaller cases were slower by as much.
 // Every wait is bounded; when one gives up, the CTA's results are not numbers.
 #include "e8_cache_attention.cuh"
 #include "umma.cuh"
@@ -29,6 +33,8 @@ namespace {
 
 constexpr int kTileRows = 128, kTile = 128;  // queries and tokens of a tile
 constexpr int kLeastPage = 16;           // tokens of a page
+// A segment's cost beyond its tiles, in tiles, and the least that a CTA does.  4 sequences of 8000 to 16384 tokens with 512 rows 194 us (2 tiles: 200, 8: 197), 32 of 3000 to
+// 6000 with 32 rows 140 (139, 145); 2 of 300 to 600 with 28 rows 17.9 us (at least 1 tile: 18.4, 4: 23.4).
 constexpr int kSegment = 4, kLeastTiles = 2;
 constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4, kProductWarp = kSoftmaxWarps + kDecodeWarps, kThreads = 32 * (kProductWarp + 1);
 constexpr float kSlack = 8.0f, kShift = 6.0f;  // weights reach 2^(1 + kSlack + kShift)
