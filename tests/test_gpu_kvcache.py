@@ -499,6 +499,32 @@ def test_starts_that_make_no_sense_touch_nothing_outside(heads, dtype):
     check(q, pages, 64, table, [40] * 3, [0, 1, 3, 6], None)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+@pytest.mark.parametrize("dim, group, dtype", [(64, 2, "f32"), (128, 2, "bf16"), (128, 24, "bf16"), (64, 70, "bf16")])
+def test_scales(dim, group, dtype, scale):
+    pages, table = filled(dim, 1, 16, [70, 33], 8)
+    q = rows(4, group, dim, 9, DTYPES[dtype]).cuda()
+    check(q, pages, dim, table, [70, 33], [0, 2, 4], None, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_broadcast_rows_and_parts_of_a_cache(dtype):
+    """Keys that all heads share are written from one copy; the pages from some page on are a cache of their own."""
+    kv = api()
+    dim, page = 128, 16
+    whole = kv.e8_cache_pages(5, 3, page, dim)
+    k, v = rows(20, 1, dim, 1, DTYPES[dtype]).cuda(), rows(20, 3, dim, 2, DTYPES[dtype]).cuda()
+    slots = torch.arange(20, device="cuda")
+    part = whole[2:]
+    kv.e8_cache_write(part, k.expand(20, 3, dim), v, slots)
+    other = kv.e8_cache_pages(3, 3, page, dim)
+    kv.e8_cache_write(other, k.expand(20, 3, dim).contiguous(), v, slots)
+    assert torch.equal(part, other) and not whole[:2].any()
+    q = rows(1, 6, dim, 3, DTYPES[dtype]).cuda()
+    t, n = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda"), torch.tensor([20], dtype=torch.int32, device="cuda")
+    assert torch.equal(kv.e8_cache_attention(q, part, t, n), kv.e8_cache_attention(q, whole, t + 2, n))
+
+
 def test_queries_in_other_orders_and_no_queries():
     kv = api()
     dim, lens = 128, [77, 20]
