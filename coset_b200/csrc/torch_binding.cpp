@@ -785,12 +785,18 @@ const Tensor& index_arg(PyObject* o, const char* name, at::ScalarType type, int6
     same_device(t, pages, name);
     return t;
 }
-// x [n, heads, dim] as rows that begin at multiples of 16 bytes
-Tensor cache_rows(const Tensor& x) {
-    const int64_t whole = 16 / x.element_size();
-    const bool fits = x.numel() == 0 || (x.stride(2) == 1 && x.stride(0) % whole == 0 && x.stride(1) % whole == 0 && (uintptr_t)x.data_ptr() % 16 == 0);
-    if (fits) return x;
-    return x.is_contiguous() ? x.clone() : x.contiguous();
+// x [n, heads, dim] as rows that begin at multiples of 16 bytes, copied where they do not.  The stride of a dimension of one may be anything: it is not looked at.
+struct CacheRows {
+    Tensor t;
+    int64_t token_stride, head_stride;
+};
+CacheRows cache_rows(const Tensor& x) {
+    const int64_t whole = 16 / x.element_size(), heads = x.size(1), dim = x.size(2);
+    const int64_t token = x.size(0) > 1 ? x.stride(0) : heads * dim, head = heads > 1 ? x.stride(1) : dim;
+    if (x.numel() == 0 || (x.stride(2) == 1 && token % whole == 0 && head % whole == 0 && (uintptr_t)x.data_ptr() % 16 == 0)) return {x, token, head};
+    Tensor copy = empty(x.sizes(), x.scalar_type(), x);
+    copy.copy_(x);
+    return {copy, heads * dim, dim};
 }
 
 // cache_write(pages, k, v, slots)
@@ -811,9 +817,10 @@ PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     {
         NoGil no_gil;
         c10::cuda::CUDAGuard guard(p.t.device());
-        const Tensor kr = cache_rows(k), vr = cache_rows(v), at = contiguous(slots);
-        check_rc(coset_e8_cache_write(data(p.t), p.n_pages, p.n_heads, p.page_size, p.dim, data(kr), kr.stride(0), kr.stride(1), data(vr), vr.stride(0),
-                                      vr.stride(1), code, (const int64_t*)data(at), k.size(0), stream_of(p.t)), "coset_e8_cache_write");
+        const CacheRows kr = cache_rows(k), vr = cache_rows(v);
+        const Tensor at = contiguous(slots);
+        check_rc(coset_e8_cache_write(data(p.t), p.n_pages, p.n_heads, p.page_size, p.dim, data(kr.t), kr.token_stride, kr.head_stride, data(vr.t),
+                                      vr.token_stride, vr.head_stride, code, (const int64_t*)data(at), k.size(0), stream_of(p.t)), "coset_e8_cache_write");
     }
     written(p.t);
     Py_RETURN_NONE;
@@ -912,14 +919,15 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     {
         NoGil no_gil;
         c10::cuda::CUDAGuard guard(p.t.device());
-        const Tensor qr = cache_rows(q), pages_of = table.stride(1) == 1 || table.size(1) <= 1 ? table : table.contiguous(), len = contiguous(lens);
+        const CacheRows qr = cache_rows(q);
+        const Tensor pages_of = table.stride(1) == 1 || table.size(1) <= 1 ? table : table.contiguous(), len = contiguous(lens);
         if (starts.defined()) starts = contiguous(starts);
         if (tree.defined()) tree = contiguous(tree);
         if (!given) out = empty(q.sizes(), q.scalar_type(), q);
         if (want_lse) lse = empty({queries, q.size(1)}, at::kFloat, q);
         const int64_t bytes = coset_e8_cache_attention_scratch_bytes(p.dim);
         const Tensor scratch = queries > 0 ? attention_scratch(bytes, q) : Tensor();
-        check_rc(coset_e8_cache_attention(data(qr), code, qr.stride(0), qr.stride(1), (int)queries, (int)q.size(1), data(p.t), p.n_pages, p.n_heads, p.page_size,
+        check_rc(coset_e8_cache_attention(data(qr.t), code, qr.token_stride, qr.head_stride, (int)queries, (int)q.size(1), data(p.t), p.n_pages, p.n_heads, p.page_size,
                                           p.dim, (const int32_t*)data(pages_of), pages_of.stride(0), (int)pages_of.size(1), (const int32_t*)data(len),
                                           starts.defined() ? (const int32_t*)data(starts) : nullptr, (int)seqs, tree.defined() ? (const int64_t*)data(tree) : nullptr,
                                           scale, data(out), want_lse ? fdata(lse) : nullptr, scratch.defined() ? scratch.data_ptr() : nullptr, bytes,
