@@ -857,26 +857,30 @@ PyObject* cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// The attention's scratch: kept for each stream, whose calls follow one another.  A capture gets one of its own, its counters cleared in the graph, so that
-// a replay shares it with no other call.
+// The attention's scratch: kept for each stream, whose calls follow one another.  Streams are told apart by their ids: a handle may stand for several, one after
+// the other, or, as that of the per-thread default stream, for one in every thread at once.  Ids are never used again, so no more than kMostKept buffers are kept
+// for a device; PyTorch's own streams are fewer, and calls on streams beyond that have a buffer each.  A capture gets one of its own, its counters cleared in
+// the graph, so that a replay shares it with no other call.
 Tensor attention_scratch(int64_t bytes, const Tensor& like) {
+    constexpr size_t kMostKept = 160;
     const auto fresh = [&]() {
         Tensor t = empty({bytes}, at::kByte, like);
         t.narrow(0, 0, std::min<int64_t>(bytes, COSET_E8_CACHE_SCRATCH_ZEROS)).zero_();
         return t;
     };
-    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(like.get_device()).stream();
     if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return fresh();
+    unsigned long long id = 0;
+    C10_CUDA_CHECK(cudaStreamGetId(c10::cuda::getCurrentCUDAStream(like.get_device()).stream(), &id));
     static std::mutex mutex;
-    static auto* kept = new std::map<std::pair<int, cudaStream_t>, Tensor>();  // never destroyed: the driver may be gone before static objects are
+    static auto* kept = new std::map<int, std::map<unsigned long long, Tensor>>();  // never destroyed: the driver may be gone before static objects are
     const std::lock_guard<std::mutex> lock(mutex);
-    Tensor& t = (*kept)[{(int)like.get_device(), stream}];
-    if (!t.defined() || t.numel() < bytes) {
-        const at::AutoDispatchBelowADInplaceOrView below;
-        const c10::InferenceMode normal(false);
-        t = fresh();
-    }
-    return t;
+    auto& its = (*kept)[like.get_device()];
+    const auto at = its.find(id);
+    if (at != its.end() && at->second.numel() >= bytes) return at->second;
+    if (at == its.end() && its.size() >= kMostKept) return fresh();
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const c10::InferenceMode normal(false);
+    return its[id] = fresh();
 }
 
 // cache_attention(q, pages, table, lens, q_starts or None, tree or None, scale, return_lse, out or None) -> out or (out, lse)

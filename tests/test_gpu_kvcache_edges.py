@@ -1,4 +1,4 @@
-"""The E8-coded key/value cache at the edges of what its calls allow: layouts with dimensions of one."""
+"""The E8-coded key/value cache at the edges of what its calls allow: layouts with dimensions of one, streams that are not PyTorch's own."""
 import os
 import sys
 
@@ -7,7 +7,7 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_gpu_kvcache import DTYPES, api, as_words, expected_pages, rows
+from test_gpu_kvcache import DTYPES, api, as_words, expected_pages, filled, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,65 @@ def test_rows_of_any_stride_where_a_dimension_is_one(dim, heads, n, dtype):
     for odd in (1, 3):
         assert torch.equal(kv.e8_cache_attention(cut_from_wider(k, odd), pages, t, lens), plainly)
     assert torch.equal(kv.e8_cache_attention(apart, pages, t, lens), plainly)
+
+
+# ------------------------------------------------------------------ streams
+def test_the_per_thread_default_stream_is_another_one_in_every_thread():
+    """One handle, a stream for each thread: calls that run at the same time share nothing.  (The threads allocate nothing between their calls: PyTorch's
+    allocator takes these streams for one.)"""
+    import threading
+    kv = api()
+    dim, calls, tokens = 128, 60, (1, 9, 40)
+    pages, table = filled(dim, 2, 16, [900, 300], 5)
+    t, n = torch.tensor(table, dtype=torch.int32, device="cuda"), torch.tensor([900, 300], dtype=torch.int32, device="cuda")
+    qs = [[rows(2 * k, 8, dim, 10 * s + k, torch.bfloat16).cuda() for k in tokens] for s in range(4)]
+    want = [[kv.e8_cache_attention(q, pages, t, n) for q in its] for its in qs]
+    outs = [[[torch.zeros_like(q) for q in its] for _ in range(calls)] for its in qs]
+    torch.cuda.synchronize()
+    start, raised = threading.Barrier(4), []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.ExternalStream(2)):  # cudaStreamPerThread
+                start.wait(30)
+                for out in outs[i]:
+                    for q, y in zip(qs[i], out):
+                        kv.e8_cache_attention(q, pages, t, n, out=y)
+        except BaseException as e:
+            raised.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    torch.cuda.synchronize()
+    assert not raised
+    for i in range(4):
+        for out in outs[i]:
+            assert all(torch.equal(y, w) for y, w in zip(out, want[i]))
+
+
+def test_streams_that_come_and_go():
+    """Streams made elsewhere, each used and destroyed: more of them than buffers are kept for, without one being held for each."""
+    import ctypes
+    kv = api()
+    dim = 64
+    pages, table = filled(dim, 2, 16, [700], 5)
+    t, n = torch.tensor(table, dtype=torch.int32, device="cuda"), torch.tensor([700], dtype=torch.int32, device="cuda")
+    q = rows(1, 8, dim, 1, torch.bfloat16).cuda()
+    want = kv.e8_cache_attention(q, pages, t, n)
+    torch.cuda.synchronize()
+    runtime, most = torch.cuda.cudart(), 0
+    for i in range(400):
+        handle = ctypes.c_void_p()
+        assert int(runtime.cudaStreamCreate(ctypes.addressof(handle))) == 0
+        with torch.cuda.stream(torch.cuda.ExternalStream(handle.value)):
+            y = kv.e8_cache_attention(q, pages, t, n)
+            torch.cuda.current_stream().synchronize()
+        assert torch.equal(y, want)
+        del y
+        assert int(runtime.cudaStreamDestroy(handle.value)) == 0
+        if i in (199, 399):
+            most = torch.cuda.memory_allocated() - (most if i == 399 else 0)
+    assert most <= 2 ** 20  # nothing is kept for the last 200
