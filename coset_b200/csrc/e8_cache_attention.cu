@@ -252,6 +252,10 @@ k_cache_attend(const __grid_constant__ Attend a) {
     using L = Layout<DIM, NB, WARPS>;
     constexpr int kRows = 8 * NB, kThreads = 32 * WARPS, kWeights = BF16 ? 1 : 2;  // 16-bit parts of a weight
     constexpr int kPart = kRows * (DIM + 2);  // floats of a CTA's part: maxima, sums, rows; it has one for a segment that began before it and one for one that goes on behind it
+    // Units after which a warp's sums are added to float32 ones in shared memory.  The tensor cores round their sums towards zero: each of a unit's two (float32
+    // queries: four) products takes some 2^-24.6 of a sum of one sign with it, so that float32 results of 131,072 tokens which one warp had were 2.7e-4 too
+    // small.  Now that is 2^-19.6 (bf16: 2^-17.6) at any length; it takes 1 us per run of a warp, 5 % of long float32 calls and 2 % of bf16 ones (all 16 units: 5 %).
+    constexpr int kRun = BF16 ? 64 : 8;
     constexpr float kSlack = BF16 ? 8.0f : 2.0f, kShift = BF16 ? 6.0f : 12.0f;  // weights reach 2^(1 + kSlack + kShift)
     extern __shared__ __align__(128) uint8_t smem[];
     auto* const all_queries = reinterpret_cast<Queries<DIM, NB>*>(smem + L::kQueries);
@@ -354,206 +358,266 @@ k_cache_attend(const __grid_constant__ Attend a) {
             m[nb][0] = m[nb][1] = kNothing;
             l[nb][0] = l[nb][1] = 0.0f;
         }
-        const int drafted = place.s.len - place.s.count;
-        for (int k = 0; k < my_units; ++k) {
-            __syncwarp();  // every lane has read the stage that is filled next
-            if ((k + L::kStages - 1) % 32 == 0) look_up(k + L::kStages - 1, n);
-            fetch(k + L::kStages - 1, my_units, stage == 0 ? L::kStages - 1 : stage - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 1) : "memory");
-            __syncwarp();
-            const uint8_t* at = smem + (warp * L::kStages + stage) * S::kStage;
-            const auto head_word = [&](int byte) { return *reinterpret_cast<const uint32_t*>(at + byte); };
-            const int token0 = (place.tile + warp + k * WARPS) * kUnit;
-
-            // scores: [group of 16 tokens][tile of 8 queries][token g: query 2 t, 2 t + 1; token g + 8: the same]
-            float s[2][NB][4], step[2][2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                int sum[kQueryBytes][NB][4];
-#pragma unroll
-                for (int j = 0; j < kQueryBytes; ++j)
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        const int2 s0 = *reinterpret_cast<const int2*>(&queries.start[j][8 * nb + 2 * t]);
-                        sum[j][nb][0] = sum[j][nb][2] = s0.x;
-                        sum[j][nb][1] = sum[j][nb][3] = s0.y;
-                    }
-                uint32_t kw[2][S::kKeyWords], kh[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int rows = (16 * h + 8 * e) * S::kRowBytes;
-                    if (DIM == 64) load_words<2>(at + key_at + rows, kw[e]);
-                    else load_words<4>(at + key_at + rows, kw[e]);
-                    if (DIM == 256) load_words<4>(at + key_at_1 + rows, kw[e] + S::kKeyWords / 2);
-                    kh[e] = head_word(head_at + (16 * h + 8 * e) * S::kHeads * 4 + (DIM == 256 ? t / 2 * 4 : 0));
-                    step[h][e] = __uint_as_float(kh[e] & 0xFFFF0000u);
-                }
-#pragma unroll
-                for (int w = 0; w < S::kKeyWords; ++w) {
-                    const uint32_t x0 = kw[0][w] & 0x0F0F0F0Fu, x1 = kw[1][w] & 0x0F0F0F0Fu, x2 = kw[0][w] >> 4 & 0x0F0F0F0Fu, x3 = kw[1][w] >> 4 & 0x0F0F0F0Fu;
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        const auto& q = queries.words[nb][w][lane];
-                        mma_bytes<true>(sum[0][nb], x0, x1, x2, x3, q[0].x, q[0].y);
-#pragma unroll
-                        for (int j = 1; j < kQueryBytes; ++j) mma_bytes<false>(sum[j][nb], x0, x1, x2, x3, q[j].x, q[j].y);
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < S::kBitTiles; ++k) {
-                    const int shift = (DIM == 64 ? 2 * t : DIM == 128 ? 4 * t : 8 * (t & 1)) + 4 * k;
-                    const uint32_t x0 = bytes_of_bits(kh[0] >> shift), x1 = bytes_of_bits(kh[1] >> shift);
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                        for (int j = 0; j < kQueryBytes; ++j) {
-                            const uint2 q = queries.blocks[nb][j][k][lane];
-                            if (j == 0) mma_bytes<true>(sum[j][nb], x0, x1, x0 * 64, x1 * 64, q.x, q.y);
-                            else mma_bytes<false>(sum[j][nb], x0, x1, x0, x1, q.x, 0);
-                        }
-                }
+        // The warp's sums so far to its place in shared memory.  ADD: onto those of the segment's earlier runs, if there are any; what the addition rounds off stays in
+        // the registers.
+        const auto deposit = [&](auto adds, bool any) {
+            constexpr bool ADD = decltype(adds)::value;
+            float keep[NB][2];
+            if (ADD) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4) {
-                        float x = __int_as_float(sum[0][nb][i4]) - kExactly;
-#pragma unroll
-                        for (int j = 1; j < kQueryBytes; ++j) x = __fmaf_rn(x, 256.0f, __int_as_float(sum[j][nb][i4]) - kExactly);
-                        s[h][nb][i4] = x;
-                    }
-            }
-
-            // softmax
-            const bool all_seen = token0 + kUnit <= drafted && (there >> 2 * stage & 3) == 3;
-            float value_step[2][2], size[2][2], lag = -INFINITY, top[NB][2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t v = head_word(head_at + (kUnit + 16 * h + 8 * e) * S::kHeads * 4);
-                    value_step[h][e] = __uint_as_float(v & 0xFFFF0000u);
-                    size[h][e] = size_of(v);
-                }
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                const float2 factor = *reinterpret_cast<const float2*>(&queries.factor[8 * nb + 2 * t]);
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        s[h][nb][2 * e] *= step[h][e] * factor.x;
-                        s[h][nb][2 * e + 1] *= step[h][e] * factor.y;
-                    }
-            }
-            if (!all_seen) {
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const uint64_t who = queries.bits[8 * nb + 2 * t + c];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int token = token0 + 16 * h + 8 * e + placed(g), j = token - drafted;
-                                const bool seen = token < place.s.len && (there >> (2 * stage + h) & 1) && (j < 0 || (a.tree ? j < 64 && (who >> j & 1) : j <= (int)who));
-                                if (!seen) s[h][nb][2 * e + c] = -INFINITY;
-                            }
-                    }
+                    for (int c = 0; c < 2; ++c) keep[nb][c] = any ? exp2_of(joining.m[8 * nb + 2 * t + c][warp] - m[nb][c]) : 0.0f;
+                __syncwarp();  // the maxima are read
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    top[nb][c] = s[0][nb][c] + size[0][0];
-                    top[nb][c] = larger(top[nb][c], s[0][nb][2 + c] + size[0][1]);
-                    top[nb][c] = larger(top[nb][c], s[1][nb][c] + size[1][0]);
-                    top[nb][c] = larger(top[nb][c], s[1][nb][2 + c] + size[1][1]);
-                    lag = larger(lag, top[nb][c] - m[nb][c]);
+                    const int r = 8 * nb + 2 * t + c;
+                    const auto put = [&](float& at, float& x) {
+                        if (!ADD) {
+                            at = x;
+                            return;
+                        }
+                        const float kept = any ? at * keep[nb][c] : 0.0f, sum = kept + x;
+                        x -= sum - kept;
+                        at = sum;
+                    };
+                    float x = l[nb][c];
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) x += __shfl_xor_sync(0xFFFFFFFFu, x, d);
+                    if (g == 0) {
+                        joining.m[r][warp] = m[nb][c];
+                        put(joining.l[r][warp], x);
+                    }
+                    l[nb][c] = g == 0 ? x : 0.0f;
+#pragma unroll
+                    for (int k = 0; k < S::kTiles; ++k) {
+                        float2& at = *reinterpret_cast<float2*>(&joining.o[warp][r][joining.at(g * (DIM / 8) + 2 * k)]);
+                        float2 its = ADD ? at : make_float2(0.0f, 0.0f);
+                        put(its.x, o[nb][k][c]);
+                        put(its.y, o[nb][k][c + 2]);
+                        at = its;
+                    }
+#pragma unroll
+                    for (int k = 0; k < S::kBitTiles; ++k) {
+                        float* const at = &joining.bits[warp][r][g * (DIM / 64) + 2 * k];
+                        put(at[0], bits[nb][k][c]);
+                        if (DIM > 64) put(at[1], bits[nb][k][c + 2]);
+                    }
                 }
-            if (__any_sync(0xFFFFFFFFu, !(lag <= kSlack + kShift))) {
+        };
+        const int drafted = place.s.len - place.s.count;
+        for (int k = 0; k < my_units;) {
+            if (k > 0) deposit(std::true_type(), k > kRun);
+            for (const int end = min(k + kRun, my_units); k < end; ++k) {
+                __syncwarp();  // every lane has read the stage that is filled next
+                if ((k + L::kStages - 1) % 32 == 0) look_up(k + L::kStages - 1, n);
+                fetch(k + L::kStages - 1, my_units, stage == 0 ? L::kStages - 1 : stage - 1);
+                asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 1) : "memory");
+                __syncwarp();
+                const uint8_t* at = smem + (warp * L::kStages + stage) * S::kStage;
+                const auto head_word = [&](int byte) { return *reinterpret_cast<const uint32_t*>(at + byte); };
+                const int token0 = (place.tile + warp + k * WARPS) * kUnit;
+
+                // scores: [group of 16 tokens][tile of 8 queries][token g: query 2 t, 2 t + 1; token g + 8: the same]
+                float s[2][NB][4], step[2][2];
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
+                for (int h = 0; h < 2; ++h) {
+                    int sum[kQueryBytes][NB][4];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float x = top[nb][c];
+                    for (int j = 0; j < kQueryBytes; ++j)
 #pragma unroll
-                        for (int d = 4; d < 32; d *= 2) x = larger(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
-                        x = larger(m[nb][c], x - kShift);
-                        const float keep = exp2_of(m[nb][c] - x);
-                        m[nb][c] = x;
-                        l[nb][c] *= keep;
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const int2 s0 = *reinterpret_cast<const int2*>(&queries.start[j][8 * nb + 2 * t]);
+                            sum[j][nb][0] = sum[j][nb][2] = s0.x;
+                            sum[j][nb][1] = sum[j][nb][3] = s0.y;
+                        }
+                    uint32_t kw[2][S::kKeyWords], kh[2];
 #pragma unroll
-                        for (int k = 0; k < S::kTiles; ++k) { o[nb][k][c] *= keep; o[nb][k][c + 2] *= keep; }
-#pragma unroll
-                        for (int k = 0; k < S::kBitTiles; ++k) { bits[nb][k][c] *= keep; bits[nb][k][c + 2] *= keep; }
+                    for (int e = 0; e < 2; ++e) {
+                        const int rows = (16 * h + 8 * e) * S::kRowBytes;
+                        if (DIM == 64) load_words<2>(at + key_at + rows, kw[e]);
+                        else load_words<4>(at + key_at + rows, kw[e]);
+                        if (DIM == 256) load_words<4>(at + key_at_1 + rows, kw[e] + S::kKeyWords / 2);
+                        kh[e] = head_word(head_at + (16 * h + 8 * e) * S::kHeads * 4 + (DIM == 256 ? t / 2 * 4 : 0));
+                        step[h][e] = __uint_as_float(kh[e] & 0xFFFF0000u);
                     }
-            }
-            uint32_t p[2][NB][2][kWeights];  // weights as 16-bit pairs of queries, [group][tile][token g, g + 8][part]
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+                    for (int w = 0; w < S::kKeyWords; ++w) {
+                        const uint32_t x0 = kw[0][w] & 0x0F0F0F0Fu, x1 = kw[1][w] & 0x0F0F0F0Fu, x2 = kw[0][w] >> 4 & 0x0F0F0F0Fu, x3 = kw[1][w] >> 4 & 0x0F0F0F0Fu;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const auto& q = queries.words[nb][w][lane];
+                            mma_bytes<true>(sum[0][nb], x0, x1, x2, x3, q[0].x, q[0].y);
 #pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4) {
-                        const float x = exp2_of(s[h][nb][i4] - m[nb][i4 & 1]);
-                        l[nb][i4 & 1] += x;
-                        s[h][nb][i4] = x * value_step[h][i4 >> 1];
-                        if (!all_seen && x == 0.0f) s[h][nb][i4] = 0.0f;  // whatever stands in a place that is not seen
+                            for (int j = 1; j < kQueryBytes; ++j) mma_bytes<false>(sum[j][nb], x0, x1, x2, x3, q[j].x, q[j].y);
+                        }
                     }
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+                    for (int k = 0; k < S::kBitTiles; ++k) {
+                        const int shift = (DIM == 64 ? 2 * t : DIM == 128 ? 4 * t : 8 * (t & 1)) + 4 * k;
+                        const uint32_t x0 = bytes_of_bits(kh[0] >> shift), x1 = bytes_of_bits(kh[1] >> shift);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int j = 0; j < kQueryBytes; ++j) {
+                                const uint2 q = queries.blocks[nb][j][k][lane];
+                                if (j == 0) mma_bytes<true>(sum[j][nb], x0, x1, x0 * 64, x1 * 64, q.x, q.y);
+                                else mma_bytes<false>(sum[j][nb], x0, x1, x0, x1, q.x, 0);
+                            }
+                    }
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int i4 = 0; i4 < 4; ++i4) {
+                            float x = __int_as_float(sum[0][nb][i4]) - kExactly;
+#pragma unroll
+                            for (int j = 1; j < kQueryBytes; ++j) x = __fmaf_rn(x, 256.0f, __int_as_float(sum[j][nb][i4]) - kExactly);
+                            s[h][nb][i4] = x;
+                        }
+                }
+
+                // softmax
+                const bool all_seen = token0 + kUnit <= drafted && (there >> 2 * stage & 3) == 3;
+                float value_step[2][2], size[2][2], lag = -INFINITY, top[NB][2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float w0 = s[h][nb][2 * e], w1 = s[h][nb][2 * e + 1];
-                        const uint32_t pair = half_pair(w0, w1);
-                        p[h][nb][e][0] = transposed(pair);
-                        if (kWeights == 2) p[h][nb][e][kWeights - 1] = transposed(rest_pair(w0, w1, pair));
+                        const uint32_t v = head_word(head_at + (kUnit + 16 * h + 8 * e) * S::kHeads * 4);
+                        value_step[h][e] = __uint_as_float(v & 0xFFFF0000u);
+                        size[h][e] = size_of(v);
                     }
-
-            // values
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t vw[4][S::kValueWords], vh[4];  // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+                for (int nb = 0; nb < NB; ++nb) {
+                    const float2 factor = *reinterpret_cast<const float2*>(&queries.factor[8 * nb + 2 * t]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int rows = 16 * h + 8 * (k >> 1);
-                    load_words<S::kValueWords>(at + (k & 1 ? value_at_1 : value_at) + rows * S::kRowBytes, vw[k]);
-                    vh[k] = head_word((k & 1 ? pair_at_1 : pair_at) + rows * S::kHeads * 4);
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            s[h][nb][2 * e] *= step[h][e] * factor.x;
+                            s[h][nb][2 * e + 1] *= step[h][e] * factor.y;
+                        }
                 }
-                const auto add = [&](float (&acc)[NB][S::kTiles][4], int tile, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                if (!all_seen) {
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                        for (int part = 0; part < kWeights; ++part) mma(acc[nb][tile], a0, a1, a2, a3, p[h][nb][0][part], p[h][nb][1][part]);
-                };
+                        for (int c = 0; c < 2; ++c) {
+                            const uint64_t who = queries.bits[8 * nb + 2 * t + c];
 #pragma unroll
-                for (int w = 0; w < S::kValueWords; ++w)
+                            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int high = 0; high < 2; ++high) {
-                        const uint32_t x = __byte_perm(vw[0][w], vw[1][w], high ? 0x7632 : 0x5410), y = __byte_perm(vw[2][w], vw[3][w], high ? 0x7632 : 0x5410);
-                        add(o, 4 * w + 2 * high, exponents.even_values(x), exponents.odd_values(x), exponents.even_values(y), exponents.odd_values(y));
-                        add(o, 4 * w + 2 * high + 1, exponents.even_values(x >> 8), exponents.odd_values(x >> 8), exponents.even_values(y >> 8), exponents.odd_values(y >> 8));
-                    }
-                const int shift = DIM == 64 ? g : DIM == 128 ? 2 * g : 4 * (g & 3);
-                const uint32_t x = __byte_perm(vh[0], vh[1], 0x5410) >> shift << 10, y = __byte_perm(vh[2], vh[3], 0x5410) >> shift << 10;
+                                for (int e = 0; e < 2; ++e) {
+                                    const int token = token0 + 16 * h + 8 * e + placed(g), j = token - drafted;
+                                    const bool seen = token < place.s.len && (there >> (2 * stage + h) & 1) && (j < 0 || (a.tree ? j < 64 && (who >> j & 1) : j <= (int)who));
+                                    if (!seen) s[h][nb][2 * e + c] = -INFINITY;
+                                }
+                        }
+                }
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int part = 0; part < kWeights; ++part)
+                    for (int c = 0; c < 2; ++c) {
+                        top[nb][c] = s[0][nb][c] + size[0][0];
+                        top[nb][c] = larger(top[nb][c], s[0][nb][2 + c] + size[0][1]);
+                        top[nb][c] = larger(top[nb][c], s[1][nb][c] + size[1][0]);
+                        top[nb][c] = larger(top[nb][c], s[1][nb][2 + c] + size[1][1]);
+                        lag = larger(lag, top[nb][c] - m[nb][c]);
+                    }
+                if (__any_sync(0xFFFFFFFFu, !(lag <= kSlack + kShift))) {
 #pragma unroll
-                        for (int k = 0; k < S::kBitTiles; ++k)
-                            mma(bits[nb][k], x & (0x04000400u << (2 * k)), x & (0x08000800u << (2 * k)), y & (0x04000400u << (2 * k)), y & (0x08000800u << (2 * k)),
-                                p[h][nb][0][part], p[h][nb][1][part]);
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float x = top[nb][c];
+#pragma unroll
+                            for (int d = 4; d < 32; d *= 2) x = larger(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
+                            x = larger(m[nb][c], x - kShift);
+                            const float keep = exp2_of(m[nb][c] - x);
+                            m[nb][c] = x;
+                            l[nb][c] *= keep;
+#pragma unroll
+                            for (int k = 0; k < S::kTiles; ++k) { o[nb][k][c] *= keep; o[nb][k][c + 2] *= keep; }
+#pragma unroll
+                            for (int k = 0; k < S::kBitTiles; ++k) { bits[nb][k][c] *= keep; bits[nb][k][c + 2] *= keep; }
+                        }
+                }
+                uint32_t p[2][NB][2][kWeights];  // weights as 16-bit pairs of queries, [group][tile][token g, g + 8][part]
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float sum[2][2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                float& its = s[h][nb][2 * e + c];
+                                const float x = exp2_of(its - m[nb][c]);
+                                sum[h][e] = x;
+                                its = x * value_step[h][e];
+                                if (!all_seen && x == 0.0f) its = 0.0f;  // whatever stands in a place that is not seen
+                            }
+                        l[nb][c] += (sum[0][0] + sum[0][1]) + (sum[1][0] + sum[1][1]);
+                    }
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float w0 = s[h][nb][2 * e], w1 = s[h][nb][2 * e + 1];
+                            const uint32_t pair = half_pair(w0, w1);
+                            p[h][nb][e][0] = transposed(pair);
+                            if (kWeights == 2) p[h][nb][e][kWeights - 1] = transposed(rest_pair(w0, w1, pair));
+                        }
+
+                // values
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t vw[4][S::kValueWords], vh[4];  // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int rows = 16 * h + 8 * (k >> 1);
+                        load_words<S::kValueWords>(at + (k & 1 ? value_at_1 : value_at) + rows * S::kRowBytes, vw[k]);
+                        vh[k] = head_word((k & 1 ? pair_at_1 : pair_at) + rows * S::kHeads * 4);
+                    }
+                    const auto add = [&](float (&acc)[NB][S::kTiles][4], int tile, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int part = 0; part < kWeights; ++part) mma(acc[nb][tile], a0, a1, a2, a3, p[h][nb][0][part], p[h][nb][1][part]);
+                    };
+#pragma unroll
+                    for (int w = 0; w < S::kValueWords; ++w)
+#pragma unroll
+                        for (int high = 0; high < 2; ++high) {
+                            const uint32_t x = __byte_perm(vw[0][w], vw[1][w], high ? 0x7632 : 0x5410), y = __byte_perm(vw[2][w], vw[3][w], high ? 0x7632 : 0x5410);
+                            add(o, 4 * w + 2 * high, exponents.even_values(x), exponents.odd_values(x), exponents.even_values(y), exponents.odd_values(y));
+                            add(o, 4 * w + 2 * high + 1, exponents.even_values(x >> 8), exponents.odd_values(x >> 8), exponents.even_values(y >> 8), exponents.odd_values(y >> 8));
+                        }
+                    const int shift = DIM == 64 ? g : DIM == 128 ? 2 * g : 4 * (g & 3);
+                    const uint32_t x = __byte_perm(vh[0], vh[1], 0x5410) >> shift << 10, y = __byte_perm(vh[2], vh[3], 0x5410) >> shift << 10;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int part = 0; part < kWeights; ++part)
+#pragma unroll
+                            for (int k = 0; k < S::kBitTiles; ++k)
+                                mma(bits[nb][k], x & (0x04000400u << (2 * k)), x & (0x08000800u << (2 * k)), y & (0x04000400u << (2 * k)), y & (0x08000800u << (2 * k)),
+                                    p[h][nb][0][part], p[h][nb][1][part]);
+                }
+                if (++stage == L::kStages) stage = 0;
             }
-            if (++stage == L::kStages) stage = 0;
         }
 
         // ---- the warps' parts into one
         const Place done = place;
         const int done_units = n, live = min(n, WARPS);  // the first `live` warps had units
+        const bool deposited = my_units > kRun;
         const bool whole = done.tile == 0 && n == done.tiles;
         at_unit += n;
         if (done.tile + n == done.tiles) at_unit += kSegment;
@@ -565,27 +629,8 @@ k_cache_attend(const __grid_constant__ Attend a) {
             my_units = begin(n);
         }
         if (warp < live) {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int r = 8 * nb + 2 * t + c;
-                    float x = l[nb][c];
-#pragma unroll
-                    for (int d = 4; d < 32; d *= 2) x += __shfl_xor_sync(0xFFFFFFFFu, x, d);
-                    if (g == 0) {
-                        joining.m[r][warp] = m[nb][c];
-                        joining.l[r][warp] = x;
-                    }
-#pragma unroll
-                    for (int k = 0; k < S::kTiles; ++k)
-                        *reinterpret_cast<float2*>(&joining.o[warp][r][joining.at(g * (DIM / 8) + 2 * k)]) = make_float2(o[nb][k][c], o[nb][k][c + 2]);
-#pragma unroll
-                    for (int k = 0; k < S::kBitTiles; ++k) {
-                        joining.bits[warp][r][g * (DIM / 64) + 2 * k] = bits[nb][k][c];
-                        if (DIM > 64) joining.bits[warp][r][g * (DIM / 64) + 2 * k + 1] = bits[nb][k][c + 2];
-                    }
-                }
+            if (deposited) deposit(std::true_type(), true);
+            else deposit(std::false_type(), false);
         }
         if (more) raw.put(a, all_queries[buffer ^ 1]);
         __syncthreads();

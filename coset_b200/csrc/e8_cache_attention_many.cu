@@ -38,6 +38,10 @@ constexpr int kLeastPage = 16;           // tokens of a page
 constexpr int kSegment = 4, kLeastTiles = 2;
 constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4, kProductWarp = kSoftmaxWarps + kDecodeWarps, kThreads = 32 * (kProductWarp + 1);
 constexpr float kSlack = 8.0f, kShift = 6.0f;  // weights reach 2^(1 + kSlack + kShift)
+// Tiles after which a group's sums are added to float32 ones in scratch memory and begin anew.  The tensor cores round their sums towards zero: each of a tile's
+// eight products takes some 2^-23.8 of a sum of one sign with it, so that results of 131,072 tokens in one CTA were 2^-10.8 too small.  Now that is 2^-14.8 at any
+// length; it takes 2 % of such calls (4 sequences of 100,000 to 120,000 tokens with 128 rows 390 us, without 383), and nothing of those with fewer tiles.
+constexpr int kRun = 64;
 
 template <int DIM, bool PAIR>
 struct Layout {
@@ -97,6 +101,18 @@ __device__ __forceinline__ uint32_t seen_of(bool tree, uint64_t who, int at) {
     }
     const int n = (int)who + 1 - at;
     return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
+}
+
+// r += kept * keep, of 32 columns; neighbouring rows' results are neighbours, the next four columns lie `rows` further
+__device__ __forceinline__ void add_kept(uint32_t (&r)[32], const float4* kept, int rows, float keep, bool any) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float4 old = any ? kept[j * rows] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        r[4 * j] = __float_as_uint(__fmaf_rn(old.x, keep, __uint_as_float(r[4 * j])));
+        r[4 * j + 1] = __float_as_uint(__fmaf_rn(old.y, keep, __uint_as_float(r[4 * j + 1])));
+        r[4 * j + 2] = __float_as_uint(__fmaf_rn(old.z, keep, __uint_as_float(r[4 * j + 2])));
+        r[4 * j + 3] = __float_as_uint(__fmaf_rn(old.w, keep, __uint_as_float(r[4 * j + 3])));
+    }
 }
 
 // join_ctas for parts of many rows: first the rows' maxima and sums, which give each part's weight (`weights`: room for ROWS floats per CTA of the launch),
@@ -178,6 +194,7 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
     using L = Layout<DIM, PAIR>;
     constexpr int kRows = L::kRows;
     constexpr int kPart = kRows * (DIM + 2), kChunks = DIM / 32;  // 16-byte chunks of a row of codes
+    static_assert(PAIR || 2 * kPart + 2 * kTileRows * (DIM + 2) <= 2 * kManyRows * (DIM + 2), "scratch memory");
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_base = smem_u32(smem_raw), base = (raw_base + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (base - raw_base);
@@ -282,12 +299,35 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
             const Two factors = two(factor, factor);
             float m = kNothing;
             Two l = two(0.0f, 0.0f);
-            bool first = true;  // of the group's tiles of this segment
+            bool first = true;  // no results of this segment in tensor memory
+            // The row's maximum, sum and results of earlier runs of tiles: with two groups of rows in the segment's part, which is written in the end only, else
+            // behind all the parts
+            float* const run = PAIR ? a.partials + ((int64_t)blockIdx.x * 2 + (place.tile > 0 ? 0 : 1)) * kPart
+                                    : a.partials + (int64_t)gridDim.x * 2 * kPart + (blockIdx.x * 2 + group) * (kTileRows * (DIM + 2));
+            float4* const results = reinterpret_cast<float4*>(run + 2 * kRows) + tile_row;
+            bool any_kept = false;
             for (int i = PAIR ? 0 : (tile_count ^ group) & 1; i < n; i += PAIR ? 1 : 2, ++turn) {
                 const int stage = (tile_count + i) & 1;
                 await(kValuesFull + stage, (uint32_t)((tile_count + i) >> 1) & 1u);  // the steps
                 await(kScoresFull + group, (uint32_t)turn & 1u);                     // and the products of this group before
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (const int before = PAIR ? i : i / 2; before > 0 && before % kRun == 0) {
+                    const float keep = any_kept ? exp2_of(run[tile_row] - m) : 0.0f;
+#pragma unroll 1
+                    for (int c = 0; c < DIM / 32; ++c) {
+                        uint32_t r[32];
+                        tmem_ld32(lanes + L::kResult + group * DIM + c * 32, r);
+                        add_kept(r, results + c * 8 * kRows, kRows, keep, any_kept);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            results[(c * 8 + j / 4) * kRows] = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+                    }
+                    const float2 sums = both(l);
+                    run[kRows + tile_row] = (any_kept ? run[kRows + tile_row] * keep : 0.0f) + (sums.x + sums.y);
+                    run[tile_row] = m;
+                    l = two(0.0f, 0.0f);
+                    any_kept = first = true;
+                }
                 const float* key_step = reinterpret_cast<const float*>(smem + L::kSteps) + stage * 3 * kTile;
                 const float *value_step = key_step + kTile, *size = value_step + kTile;
                 const int at0 = (place.tile + i) * kTile - drafted;
@@ -339,6 +379,7 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
                         }
                     }
                     const Two less = two(-m, -m);
+                    Two sum = two(0.0f, 0.0f);
 #pragma unroll 1
                     for (int c = 0; c < kTile / 32; ++c) {
                         const uint32_t seen = seen_in(c);
@@ -356,7 +397,7 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
                                     if (!(seen >> (j + e + 1) & 1)) t.y = -INFINITY;
                                 }
                                 const Two x = two(exp2_of(t.x), exp2_of(t.y));
-                                l = add2(l, x);
+                                sum = add2(sum, x);
                                 float2 v = both(mul2(x, e ? two(z.z, z.w) : two(z.x, z.y)));
                                 if (!kAll) {  // whatever stands in a place that is not seen
                                     if (!(seen >> (j + e) & 1)) v.x = 0.0f;
@@ -367,6 +408,7 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
                         }
                         tmem_st16(scores + c * 16, w);  // over scores that are read
                     }
+                    l = add2(l, sum);
                 };
                 if (__any_sync(0xFFFFFFFFu, gap)) softmax(std::false_type());
                 else softmax(std::true_type());
@@ -380,6 +422,22 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
             const float2 sums = both(l);
             float sum = sums.x + sums.y;
             if (!first) await(kResultDone + group, (uint32_t)(turn - 1) & 1u);
+            if (any_kept) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const float keep = exp2_of(run[tile_row] - m);
+                sum += run[kRows + tile_row] * keep;
+#pragma unroll 1
+                for (int c = 0; c < DIM / 32; ++c) {
+                    uint32_t r[32];
+                    const uint32_t at = lanes + L::kResult + group * DIM + c * 32;
+                    tmem_ld32(at, r);
+                    add_kept(r, results + c * 8 * kRows, kRows, keep, true);
+                    tmem_st16(at, r);
+                    tmem_st16(at + 16, r + 16);
+                }
+                tmem_stored();
+                if (PAIR) sync_softmax();  // all of it is read before the part is written: the groups have the same tiles
+            }
             float keeps[2] = {1.0f, 1.0f};
             if (!PAIR) {
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -599,7 +657,7 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
 #pragma unroll
                         for (int k = 0; k < kTile / 16; ++k)  // 16 tokens: two groups of eight lines of a panel
                             umma_f16_from_tmem(tmem + L::kResult + group * DIM, tmem + group * kTile + k * 8, make_desc(values + stage * (L::kOperand >> 4) + k * 128, high),
-                                               kResultDesc, i > 2 || k > 0);
+                                               kResultDesc, (i - 1) / 2 % kRun > 0 || k > 0);
                         umma_commit(bar(kResultDone + group));
                         if (!PAIR || group == 1) umma_commit(bar(kValuesEmpty + stage));
                     }

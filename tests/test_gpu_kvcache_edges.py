@@ -1,4 +1,5 @@
-"""The E8-coded key/value cache at the edges of what its calls allow: layouts with dimensions of one, streams that are not PyTorch's own."""
+"""The E8-coded key/value cache at the edges of what its calls allow: layouts with dimensions of one, streams that are not PyTorch's own, long sums."""
+import math
 import os
 import sys
 
@@ -107,3 +108,54 @@ def test_streams_that_come_and_go():
         if i in (199, 399):
             most = torch.cuda.memory_allocated() - (most if i == 399 else 0)
     assert most <= 2 ** 20  # nothing is kept for the last 200
+
+
+# ------------------------------------------------------------------ long sums
+LONG = [("f32", 128, 1, 1), ("f32", 64, 2, 5), ("f32", 256, 1, 1), ("bf16", 128, 4, 1), ("bf16", 128, 4, 3), ("bf16", 256, 2, 1), ("bf16", 64, 8, 5), ("bf16", 64, 8, 32),
+        ("bf16", 128, 8, 16), ("bf16", 128, 8, 32)]
+
+
+@pytest.mark.parametrize("alike", [4096, 262144], ids=["keys in groups", "keys alike"])
+@pytest.mark.parametrize("form", LONG, ids=lambda f: f"{f[0]}d{f[1]}g{f[2]}t{f[3]}")
+def test_sums_over_long_sequences(form, alike):
+    """More sequences than the chip has CTAs, so that one CTA sums 262144 tokens.  Where the values are the same for all tokens, or follow no key, the result is
+    their mean whatever the weights are: scores' errors leave no trace, weights' roundings at most 2^-11 (bf16 queries: half a step of 11 bits) or 2^-22 of it, and the sums of
+    weights and of results are to be float32 sums, which is 2^-18.  The mean of a bf16 result lies 2^-10 beside the border between two numbers: further than all of it."""
+    dtype, dim, group, tokens = form
+    kv = api()
+    L, page, heads, seqs = 262144, 128, 2, 160
+    pages = kv.e8_cache_pages(L // page, heads, page, dim)
+    g = torch.Generator().manual_seed(7)
+    k = rows((L + alike - 1) // alike, heads, dim, 1).repeat_interleave(alike, 0)[:L].clone()
+    if alike > 4096:
+        k[:256] *= 0.5  # the running maximum is another one than that of most
+    table = torch.arange(L // page, dtype=torch.int32, device="cuda").expand(seqs, -1)
+    lens = torch.full((seqs,), L, dtype=torch.int32, device="cuda")
+    q = rows(tokens, heads * group, dim, 2, DTYPES[dtype]).cuda()
+    slots = torch.arange(L, device="cuda")
+    border = 7.0 - 2.0 ** -6  # between two bf16 numbers, 2^-5 apart
+    for mean in ((6.5,) if dtype == "f32" else (border * (1 - 2.0 ** -10), border * (1 + 2.0 ** -10))):
+        sevens = round((mean - 6) * 4096)  # of 4096 tokens in a row
+        place = torch.arange(L) % 4096
+        v = torch.where((place + 1) * sevens // 4096 > place * sevens // 4096, 7.0, 6.0)[:, None, None].expand(L, heads, dim).clone()
+        v[..., 0] = 7.0  # a step of 1
+        if dtype == "f32":
+            v[:] = 7.0 * (1 + torch.rand(1, heads, dim, generator=g))
+        kv.e8_cache_write(pages, k.cuda(), v.cuda(), slots)
+        y, z = kv.e8_cache_attention(q.repeat(seqs, 1, 1), pages, table, lens, return_lse=True, tree=torch.full((seqs * tokens,), -1, device="cuda"))
+        y, z = y.view(seqs, tokens, heads, group, dim), z.view(seqs, tokens, heads, group)
+        kd, vd = (x.double() for x in kv.e8_cache_read(pages, slots))
+        if dtype == "f32":
+            worst = float((y.double() / vd[0, :, None] - 1).abs().max())
+            assert worst <= 2.0 ** -24 + 2 * 2.0 ** -22 + 2.0 ** -18, f"{worst} of the mean"
+        else:
+            assert abs(float(vd[:, 0, 1].mean()) - mean) < 2.0 ** -13 and (vd[..., 1:8] == vd[..., 1:2]).all()
+            want = 7.0 if mean > border else 7.0 - 2.0 ** -5
+            part = float((y[..., 1:8].float() != want).float().mean())
+            assert part == 0.0, f"{part} of the results are on the wrong side"
+        s = torch.einsum("thgd,nhd->thgn", q.double().view(tokens, heads, group, dim), kd) / math.sqrt(dim)
+        reach = torch.einsum("thgd,nhd->thgn", q.double().abs().view(tokens, heads, group, dim), kd.abs()[::128]).amax(-1) / math.sqrt(dim)
+        lse = torch.logsumexp(s, -1)
+        bound = (2.0 ** -22 + (dim + 32) * 2.0 ** -24) * 4 * reach + 2.0 ** -20 + 2.0 ** -18 + 2.0 ** -22 * lse.abs()
+        worst = float(((z.double() - lse) / bound).abs().max())
+        assert worst <= 1.0, f"lse: {worst} of the bound"
