@@ -362,12 +362,12 @@ k_cache_attend(const __grid_constant__ Attend a) {
         // the registers.
         const auto deposit = [&](auto adds, bool any) {
             constexpr bool ADD = decltype(adds)::value;
-            float keep[NB][2];
+            float by[NB][2] = {};
             if (ADD) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) keep[nb][c] = any ? exp2_of(joining.m[8 * nb + 2 * t + c][warp] - m[nb][c]) : 0.0f;
+                    for (int c = 0; c < 2; ++c) by[nb][c] = any ? joining.m[8 * nb + 2 * t + c][warp] - m[nb][c] : 0.0f;
                 __syncwarp();  // the maxima are read
             }
 #pragma unroll
@@ -375,21 +375,19 @@ k_cache_attend(const __grid_constant__ Attend a) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int r = 8 * nb + 2 * t + c;
-                    const auto put = [&](float& at, float& x) {
-                        if (!ADD) {
-                            at = x;
-                            return;
-                        }
-                        const float kept = any ? at * keep[nb][c] : 0.0f, sum = kept + x;
+                    const Keep keep(by[nb][c]);
+                    const auto sum_of = [&](float kept, float& x) {
+                        const float sum = kept + x;
                         x -= sum - kept;
-                        at = sum;
+                        return sum;
                     };
+                    const auto put = [&](float& at, float& x) { at = ADD ? sum_of(any ? at * keep.factor() : 0.0f, x) : x; };
                     float x = l[nb][c];
 #pragma unroll
                     for (int d = 4; d < 32; d *= 2) x += __shfl_xor_sync(0xFFFFFFFFu, x, d);
                     if (g == 0) {
                         joining.m[r][warp] = m[nb][c];
-                        put(joining.l[r][warp], x);
+                        joining.l[r][warp] = ADD ? sum_of(any ? keep.of_sum(joining.l[r][warp]) : 0.0f, x) : x;
                     }
                     l[nb][c] = g == 0 ? x : 0.0f;
 #pragma unroll
@@ -536,9 +534,10 @@ k_cache_attend(const __grid_constant__ Attend a) {
 #pragma unroll
                             for (int d = 4; d < 32; d *= 2) x = larger(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
                             x = larger(m[nb][c], x - kShift);
-                            const float keep = exp2_of(m[nb][c] - x);
+                            const Keep kept(m[nb][c] - x);
+                            const float keep = kept.factor();
                             m[nb][c] = x;
-                            l[nb][c] *= keep;
+                            l[nb][c] = kept.of_sum(l[nb][c]);
 #pragma unroll
                             for (int k = 0; k < S::kTiles; ++k) { o[nb][k][c] *= keep; o[nb][k][c + 2] *= keep; }
 #pragma unroll
@@ -644,14 +643,15 @@ k_cache_attend(const __grid_constant__ Attend a) {
             float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll 1
             for (int w = 0; w < live; ++w) {
-                const float keep = exp2_of(joining.m[r][w] - highest);
+                const Keep kept(joining.m[r][w] - highest);
+                const float keep = kept.factor();
                 if (keep != 0.0f) {  // a warp that saw nothing has nothing to add, whatever the row's maximum is
                     const float2 x = *reinterpret_cast<const float2*>(&joining.o[w][r][joining.at(d)]);
                     const float half = joining.bits[w][r][d / 8] * half_of_bit<DIM>(d / 8);
                     v.x += (x.x + half) * keep;
                     v.y += (x.y + half) * keep;
-                    sum += joining.l[r][w] * keep;
                 }
+                sum += kept.of_sum(joining.l[r][w]);
             }
             if (whole) {
                 const float part_of = highest == kNothing ? 0.0f : 1.0f / sum;

@@ -76,6 +76,14 @@ __device__ __forceinline__ float exp2_of(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 2^by, by <= 0, for results and for sums whose maximum is -by below another.  Maxima count a value's size, so that sums of weights range over 200 powers of two, and
+// tokens whose values are zeros may have a share in one whose maximum is 2^130 above theirs: 2^by may be no number any more where the sum times it is one.
+struct Keep {
+    float half;
+    __device__ __forceinline__ explicit Keep(float by) : half(exp2_of(0.5f * by)) {}
+    __device__ __forceinline__ float factor() const { return half * half; }
+    __device__ __forceinline__ float of_sum(float sum) const { return sum * half * half; }
+};
 // (x & mask) | bits in one instruction, of which the compiler makes two when it knows both constants
 __device__ __forceinline__ uint32_t chosen(uint32_t x, uint32_t mask, uint32_t bits) {
     uint32_t d;
@@ -245,17 +253,20 @@ __device__ __forceinline__ void join_ctas(const Attend& a, Pending* pending, int
                 float higher = highest;
 #pragma unroll
                 for (int k = 0; k < kAtOnce; ++k) higher = larger(higher, m_of[k]);
-                const float before = exp2_of(highest - higher);
+                const Keep kept(highest - higher);
+                const float before = kept.factor();
                 v.x *= before; v.y *= before; v.z *= before; v.w *= before;
-                sum *= before;
+                sum = kept.of_sum(sum);
                 highest = higher;
 #pragma unroll
                 for (int k = 0; k < kAtOnce; ++k) {
-                    const float keep = i0 + k < parts ? exp2_of(m_of[k] - highest) : 0.0f;
+                    if (i0 + k >= parts) continue;
+                    const Keep kept(m_of[k] - highest);
+                    const float keep = kept.factor();
                     if (keep != 0.0f) {
                         v.x += x[k].x * keep; v.y += x[k].y * keep; v.z += x[k].z * keep; v.w += x[k].w * keep;
-                        sum += l_of[k] * keep;
                     }
+                    sum += kept.of_sum(l_of[k]);
                 }
             }
             const float part_of = highest == kNothing ? 0.0f : 1.0f / sum;

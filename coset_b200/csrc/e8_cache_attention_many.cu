@@ -141,7 +141,7 @@ __device__ __forceinline__ void join_many(const Attend& a, Pending* pending, int
             for (int k = 0; k < parts; ++k) {
                 const float* part = part_at(first_cta, k);
                 const float m = __ldcg(part + r), l = __ldcg(part + ROWS + r), higher = larger(highest, m);
-                sum = sum * exp2_of(highest - higher) + l * exp2_of(m - higher);
+                sum = Keep(highest - higher).of_sum(sum) + Keep(m - higher).of_sum(l);
                 highest = higher;
                 weights[k * ROWS + r] = m;
             }
@@ -312,18 +312,18 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
                 await(kScoresFull + group, (uint32_t)turn & 1u);                     // and the products of this group before
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (const int before = PAIR ? i : i / 2; before > 0 && before % kRun == 0) {
-                    const float keep = any_kept ? exp2_of(run[tile_row] - m) : 0.0f;
+                    const Keep kept(any_kept ? run[tile_row] - m : 0.0f);
 #pragma unroll 1
                     for (int c = 0; c < DIM / 32; ++c) {
                         uint32_t r[32];
                         tmem_ld32(lanes + L::kResult + group * DIM + c * 32, r);
-                        add_kept(r, results + c * 8 * kRows, kRows, keep, any_kept);
+                        add_kept(r, results + c * 8 * kRows, kRows, kept.factor(), any_kept);
 #pragma unroll
                         for (int j = 0; j < 32; j += 4)
                             results[(c * 8 + j / 4) * kRows] = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
                     }
                     const float2 sums = both(l);
-                    run[kRows + tile_row] = (any_kept ? run[kRows + tile_row] * keep : 0.0f) + (sums.x + sums.y);
+                    run[kRows + tile_row] = (any_kept ? kept.of_sum(run[kRows + tile_row]) : 0.0f) + (sums.x + sums.y);
                     run[tile_row] = m;
                     l = two(0.0f, 0.0f);
                     any_kept = first = true;
@@ -362,9 +362,9 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
                     }
                     top = larger(top, top2);
                     if (__any_sync(0xFFFFFFFFu, !(top - m <= kSlack + kShift))) {
-                        const float higher = larger(m, top - kShift), keep = exp2_of(m - higher);
+                        const float higher = larger(m, top - kShift), keep_half = Keep(m - higher).half, keep = keep_half * keep_half;
                         m = higher;
-                        l = mul2(l, two(keep, keep));
+                        l = mul2(mul2(l, two(keep_half, keep_half)), two(keep_half, keep_half));
                         if (!first) {
 #pragma unroll 1
                             for (int c = 0; c < DIM / 32; ++c) {
@@ -424,14 +424,14 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
             if (!first) await(kResultDone + group, (uint32_t)(turn - 1) & 1u);
             if (any_kept) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const float keep = exp2_of(run[tile_row] - m);
-                sum += run[kRows + tile_row] * keep;
+                const Keep kept(run[tile_row] - m);
+                sum += kept.of_sum(run[kRows + tile_row]);
 #pragma unroll 1
                 for (int c = 0; c < DIM / 32; ++c) {
                     uint32_t r[32];
                     const uint32_t at = lanes + L::kResult + group * DIM + c * 32;
                     tmem_ld32(at, r);
-                    add_kept(r, results + c * 8 * kRows, kRows, keep, true);
+                    add_kept(r, results + c * 8 * kRows, kRows, kept.factor(), true);
                     tmem_st16(at, r);
                     tmem_st16(at + 16, r + 16);
                 }
@@ -446,9 +446,10 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
                 sync_softmax();
                 const float2 x0 = joined[0], x1 = joined[kTileRows];
                 m = larger(x0.x, x1.x);
-                keeps[0] = exp2_of(x0.x - m);
-                keeps[1] = exp2_of(x1.x - m);
-                sum = x0.y * keeps[0] + x1.y * keeps[1];
+                const Keep kept0(x0.x - m), kept1(x1.x - m);
+                keeps[0] = kept0.factor();
+                keeps[1] = kept1.factor();
+                sum = kept0.of_sum(x0.y) + kept1.of_sum(x1.y);
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const bool whole = place.tile == 0 && n == place.tiles, failed = *lost != 0;

@@ -1,4 +1,5 @@
-"""The E8-coded key/value cache at the edges of what its calls allow: layouts with dimensions of one, streams that are not PyTorch's own, long sums."""
+"""The E8-coded key/value cache at the edges of what its calls allow: layouts with dimensions of one, streams that are not PyTorch's own, long sums, values
+of every size beside each other."""
 import math
 import os
 import sys
@@ -8,7 +9,7 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_gpu_kvcache import DTYPES, api, as_words, expected_pages, filled, rows
+from test_gpu_kvcache import DTYPES, api, as_words, check, expected_pages, filled, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -159,3 +160,43 @@ def test_sums_over_long_sequences(form, alike):
         bound = (2.0 ** -22 + (dim + 32) * 2.0 ** -24) * 4 * reach + 2.0 ** -20 + 2.0 ** -18 + 2.0 ** -22 * lse.abs()
         worst = float(((z.double() - lse) / bound).abs().max())
         assert worst <= 1.0, f"lse: {worst} of the bound"
+
+
+# ------------------------------------------------------------------ sizes
+FORMS = [("f32", 64, 2), ("f32", 256, 9), ("bf16", 128, 2), ("bf16", 128, 12), ("bf16", 256, 4), ("bf16", 128, 24), ("bf16", 64, 40), ("bf16", 128, 72)]
+FORM = lambda f: f"{f[0]}d{f[1]}g{f[2]}"  # noqa: E731
+
+
+def with_values(dim, L, v, page=16, seed=3):
+    """One sequence of L tokens and one head: random keys, these values [L, dim]."""
+    kv = api()
+    pages, table = filled(dim, 1, page, [L], seed)
+    slots = torch.tensor([table[0][i // page] * page + i % page for i in range(L)], device="cuda")
+    kv.e8_cache_write(pages, rows(L, 1, dim, 30).cuda(), v.view(L, 1, dim).cuda(), slots)
+    return pages, table
+
+
+@pytest.mark.parametrize("form", FORMS, ids=FORM)
+def test_a_cache_of_zero_values_gives_zeros(form):
+    dtype, dim, group = form
+    L = 200
+    pages, table = with_values(dim, L, torch.zeros(L, dim))
+    q = (rows(2, group, dim, 32) * 6).to(DTYPES[dtype]).cuda()
+    got = check(q, pages, dim, table, [L], [0, 2], None)
+    assert not got[0].any()
+
+
+@pytest.mark.parametrize("order", ["zeros first", "zeros last", "in turn"])
+@pytest.mark.parametrize("small, large", [(0.0, 1e5), (0.0, 1e14), (0.0, 1e30), (1e-28, 1e12)])
+@pytest.mark.parametrize("form", FORMS, ids=FORM)
+def test_values_that_weigh_nothing_count_in_the_sum(form, small, large, order):
+    """Runs of tokens whose values are zeros (as of tokens that only take up attention) or tiny, beside runs of large ones: the first run's share of the
+    softmax's sum is as large as the second's."""
+    dtype, dim, group = form
+    L = 1024
+    run = torch.arange(L) // 128 if order == "in turn" else torch.arange(L) // (L // 2)
+    tiny = run % 2 == (1 if order == "zeros last" else 0)
+    v = rows(L, 1, dim, 31)[:, 0].clamp(-3, 3) * torch.where(tiny, small, large)[:, None]
+    pages, table = with_values(dim, L, v, page=64)
+    q = rows(2, group, dim, 32, DTYPES[dtype]).cuda()
+    check(q, pages, dim, table, [L], [0, 2], None)
