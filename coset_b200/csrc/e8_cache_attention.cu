@@ -560,7 +560,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
                                 its = x * value_step[h][e];
                                 if (!all_seen && x == 0.0f) its = 0.0f;  // whatever stands in a place that is not seen
                             }
-                        l[nb][c] += (sum[0][0] + sum[0][1]) + (sum[1][0] + sum[1][1]);
+                        l[nb][c] = __fmaf_rn((sum[0][0] + sum[0][1]) + (sum[1][0] + sum[1][1]), kSumUnit, l[nb][c]);
                     }
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
@@ -654,7 +654,7 @@ k_cache_attend(const __grid_constant__ Attend a) {
                 sum += kept.of_sum(joining.l[r][w]);
             }
             if (whole) {
-                const float part_of = highest == kNothing ? 0.0f : 1.0f / sum;
+                const float part_of = highest == kNothing ? 0.0f : kSumUnit / sum;
                 put_pair<BF16, DIM>(a, done, kRows, r, d, v.x * part_of, v.y * part_of);
                 if (d == 0) put_lse(a, done, kRows, r, highest, sum);
             } else {

@@ -56,7 +56,10 @@ __device__ __forceinline__ int page_of(const Attend& a, int b, int token, int le
 }
 
 constexpr float kNothing = -3.402823466e38f;  // running maximum of a row that has seen nothing
-constexpr int kLeastSize = -90;   // exponent of a value's step as far as the running maximum goes: sums of p / 2^kLeastSize stay finite
+// Exponent of a value's step as far as the running maximum goes: that of the smallest row that is kept.  A weight thus reaches 2^(1 + kSlack + kShift + 103), and sums
+// count in units of 2^13 of them: they stay finite for 2^24 tokens whose values are all that small, and for any number of larger ones.
+constexpr int kLeastSize = -103;
+constexpr float kSumUnit = 0x1p-13f;
 constexpr float kExactly = 12582912.0f;  // 1.5 2^23, to whose last bits small whole numbers are added
 // Scratch memory: a counter per CTA, zero between launches, and two parts per CTA of the rows of a tile: maxima, sums, results
 constexpr int kMostCtas = 304, kFewRows = 16, kManyRows = 256, kManyCtas = 152;
@@ -144,7 +147,8 @@ __device__ __forceinline__ void put_pair(const Attend& a, const Place& p, int ro
     else *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(x, y);
 }
 __device__ __forceinline__ void put_lse(const Attend& a, const Place& p, int rows, int r, float highest, float sum) {
-    if (a.lse) a.lse[result_row(a, p, rows, r)] = highest == kNothing ? -INFINITY : (highest + log2f(sum)) * 0.69314718f;
+    const float size = sum < 1.0f ? log2f(sum * (1.0f / kSumUnit)) : log2f(sum) + 13.0f;
+    if (a.lse) a.lse[result_row(a, p, rows, r)] = highest == kNothing ? -INFINITY : (highest + size) * 0.69314718f;
 }
 
 // What a CTA does of a launch: segments, each a (sequence, head, tile of ROWS queries) with its units of UNIT tokens and, in the cut, SEGMENT more for
@@ -269,7 +273,7 @@ __device__ __forceinline__ void join_ctas(const Attend& a, Pending* pending, int
                     sum += kept.of_sum(l_of[k]);
                 }
             }
-            const float part_of = highest == kNothing ? 0.0f : 1.0f / sum;
+            const float part_of = highest == kNothing ? 0.0f : kSumUnit / sum;
             put_pair<BF16, DIM>(a, done, ROWS, r, d, v.x * part_of, v.y * part_of);
             put_pair<BF16, DIM>(a, done, ROWS, r, d + 2, v.z * part_of, v.w * part_of);
             if (d == 0) put_lse(a, done, ROWS, r, highest, sum);

@@ -145,7 +145,7 @@ __device__ __forceinline__ void join_many(const Attend& a, Pending* pending, int
                 highest = higher;
                 weights[k * ROWS + r] = m;
             }
-            const float part_of = highest == kNothing ? 0.0f : 1.0f / sum;
+            const float part_of = highest == kNothing ? 0.0f : kSumUnit / sum;
             for (int k = 0; k < parts; ++k) weights[k * ROWS + r] = exp2_of(weights[k * ROWS + r] - highest) * part_of;
             put_lse(a, done, ROWS, r, highest, sum);
         }
@@ -408,7 +408,7 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
                         }
                         tmem_st16(scores + c * 16, w);  // over scores that are read
                     }
-                    l = add2(l, sum);
+                    l = fma2(sum, two(kSumUnit, kSumUnit), l);
                 };
                 if (__any_sync(0xFFFFFFFFu, gap)) softmax(std::false_type());
                 else softmax(std::true_type());
@@ -454,7 +454,7 @@ k_cache_attend_many(const __grid_constant__ Attend a) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const bool whole = place.tile == 0 && n == place.tiles, failed = *lost != 0;
             if (failed) sum = __uint_as_float(0x7FC00000u);
-            const float part_of = m == kNothing && !failed ? 0.0f : 1.0f / sum;
+            const float part_of = m == kNothing && !failed ? 0.0f : kSumUnit / sum;
             float* partial = a.partials + ((int64_t)blockIdx.x * 2 + (place.tile > 0 ? 0 : 1)) * kPart;
             const int64_t result = real ? result_row(a, place, kRows, tile_row) * DIM : 0;
             const int only = PAIR ? group : n == 1 ? tile_count & 1 : -1;  // the group with all results

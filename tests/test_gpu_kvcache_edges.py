@@ -200,3 +200,38 @@ def test_values_that_weigh_nothing_count_in_the_sum(form, small, large, order):
     pages, table = with_values(dim, L, v, page=64)
     q = rows(2, group, dim, 32, DTYPES[dtype]).cuda()
     check(q, pages, dim, table, [L], [0, 2], None)
+
+
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -99, 1e-29, 1e-28, 1e-26, 1e28])
+@pytest.mark.parametrize("form", FORMS, ids=FORM)
+def test_many_small_weights_beside_a_large_one(form, size):
+    """The first token weighs 2^10 to 2^26 times as much as each of the 131071 others, whose sum counts all the same, for values of every size.  All values are the
+    same: results are that, but for weights' roundings (2^-11 for bf16 queries, 2^-22 else), float32 sums (2^-18), what each weight lacks below 2^-31 of the largest,
+    and, in the run of tokens that the tensor cores sum up with the first one, 2^-23 of the sum per token: they line up products by the largest number and cut off
+    what lies behind its 24 bits.  A run is 8 units of 32 tokens for float32 queries, 64 of them or 64 tiles of 128 tokens for bf16."""
+    dtype, dim, group = form
+    kv = api()
+    L, page, heads, seqs = 131072, 128, 2, 160
+    run = 256 if dtype == "f32" else 8192
+    pages = kv.e8_cache_pages(L // page, heads, page, dim)
+    k = torch.zeros(L, heads, dim)
+    k[0, :, :2] = 7.0
+    v = (rows(1, heads, dim, 4).clamp(-3, 3) * size).expand(L, heads, dim)
+    kv.e8_cache_write(pages, k.cuda(), v.cuda(), torch.arange(L, device="cuda"))
+    vd = kv.e8_cache_read(pages, torch.arange(1, device="cuda"))[1][0].cpu().double()
+    more = torch.linspace(10, 26, heads * group).double()
+    q = torch.zeros(heads * group, dim)
+    q[:, :2] = (more * math.log(2) * math.sqrt(dim) / 14)[:, None]
+    q = q.to(DTYPES[dtype]).cuda()
+    table = torch.arange(L // page, dtype=torch.int32, device="cuda").expand(seqs, -1)
+    y, z = kv.e8_cache_attention(q.expand(seqs, -1, -1), pages, table, torch.full((seqs,), L, dtype=torch.int32, device="cuda"), return_lse=True)
+    want = vd.repeat_interleave(group, 0)
+    weight = 2.0 ** -11 if dtype == "bf16" else 2.0 ** -22
+    off = (y.cpu().double() - want).abs() / want.abs().clamp(min=1e-300)
+    worst = float(torch.where(want == 0, y.cpu().double().abs(), off).max())
+    assert worst <= torch.finfo(DTYPES[dtype]).eps / 2 + 2 * weight + 2.0 ** -18 + L * 2.0 ** -31 + run * 2.0 ** -23, f"{worst} of the value"
+    s = q[:, 0].cpu().double() * 14 / math.sqrt(dim)
+    lse = torch.logaddexp(s, torch.full_like(s, math.log(L - 1)))
+    bound = (2.0 ** -22 + (dim + 32) * 2.0 ** -24) * 4 * s + 2.0 ** -20 + 2.0 ** -18 + 2.0 ** -22 * lse
+    worst = float(((z.cpu().double() - lse).abs() / bound).max())
+    assert worst <= 1.0, f"lse: {worst} of the bound"
