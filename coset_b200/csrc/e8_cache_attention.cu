@@ -24,7 +24,7 @@
 // order of the CTAs.
 //
 // The running maximum is that of a weight times the size of its value (s + the exponent of the value's step), so that w = p step fits 16 bits: what is
-// lost is below 2^-31 of the row's largest.  It follows only when it lags by 2^kSlack.  For float32 queries w is split into two 16-bit numbers.
+// lost is below 2^-31 of the row's largest (of a run of tokens that the tensor cores sum up, 2^-23 of the sum per token: they cut off what lies behind its 24 bits).  It follows only when it lags by 2^kSlack.  For float32 queries w is split into two 16-bit numbers.
 //
 // Measured, 8 heads of 128, 4 bf16 rows each: 32 sequences of 6144 tokens 62 us, of 12,288 112, of 24,576 210, so 4.4 TB/s of codes (two thirds of the copy rate)
 // beyond 13 us that a launch, the cut, the first loads and two joins cost.  A unit takes 700 instructions (values 250, keys 160, softmax 125, fetching 60): issue slots

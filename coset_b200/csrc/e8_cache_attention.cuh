@@ -57,7 +57,9 @@ __device__ __forceinline__ int page_of(const Attend& a, int b, int token, int le
 
 constexpr float kNothing = -3.402823466e38f;  // running maximum of a row that has seen nothing
 // Exponent of a value's step as far as the running maximum goes: that of the smallest row that is kept.  A weight thus reaches 2^(1 + kSlack + kShift + 103), and sums
-// count in units of 2^13 of them: they stay finite for 2^24 tokens whose values are all that small, and for any number of larger ones.
+// count in units of 2^13 of them: they stay finite for 2^24 tokens whose values are all that small, and for any number of larger ones.  At the other end the
+// largest weight is 2^(kShift - e) beside a step of 2^e, and what lies below 2^-126 is lost: 2^-29 of it for e = 103.  (A branch to exponentials with subnormal
+// results and other units there kept all, and took 2 to 4 % of every call.)
 constexpr int kLeastSize = -103;
 constexpr float kSumUnit = 0x1p-13f;
 constexpr float kExactly = 12582912.0f;  // 1.5 2^23, to whose last bits small whole numbers are added

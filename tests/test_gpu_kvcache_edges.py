@@ -176,6 +176,19 @@ def with_values(dim, L, v, page=16, seed=3):
     return pages, table
 
 
+@pytest.mark.parametrize("size", [2.0 ** -99, 1e-30, 1e-28, 1e-26, 1e-20, 1e20, 1e30, 1e32])
+@pytest.mark.parametrize("form", FORMS, ids=FORM)
+def test_values_of_every_size(form, size):
+    """All of a sequence's values of one size, from the smallest rows that are kept to the largest whose weights keep all their bits."""
+    dtype, dim, group = form
+    L = 300
+    v = rows(L, 1, dim, 31)[:, 0]
+    v = v / v.abs().amax(-1, keepdim=True) * (1.0 + torch.rand(L, 1, generator=torch.Generator().manual_seed(2))) * size * 2.0
+    pages, table = with_values(dim, L, v)
+    q = rows(2, group, dim, 32, DTYPES[dtype]).cuda()
+    check(q, pages, dim, table, [L], [0, 2], None)
+
+
 @pytest.mark.parametrize("form", FORMS, ids=FORM)
 def test_a_cache_of_zero_values_gives_zeros(form):
     dtype, dim, group = form
@@ -202,7 +215,7 @@ def test_values_that_weigh_nothing_count_in_the_sum(form, small, large, order):
     check(q, pages, dim, table, [L], [0, 2], None)
 
 
-@pytest.mark.parametrize("size", [1.0, 2.0 ** -99, 1e-29, 1e-28, 1e-26, 1e28])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -99, 1e-29, 1e-28, 1e-26, 1e28, 1e30])
 @pytest.mark.parametrize("form", FORMS, ids=FORM)
 def test_many_small_weights_beside_a_large_one(form, size):
     """The first token weighs 2^10 to 2^26 times as much as each of the 131071 others, whose sum counts all the same, for values of every size.  All values are the
