@@ -21,6 +21,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <map>
 #include <mutex>
 
@@ -883,7 +884,7 @@ Tensor attention_scratch(int64_t bytes, const Tensor& like) {
     return its[id] = fresh();
 }
 
-// cache_attention(q, pages, table, lens, q_starts or None, tree or None, scale, return_lse, out or None) -> out or (out, lse)
+// cache_attention(q, pages, table, lens, q_starts or None, tree or None, scale or None, return_lse, out or None) -> out or (out, lse)
 PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     nargs_are(n, 9);
@@ -909,7 +910,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         TORCH_CHECK_VALUE(tree.size(0) == queries, "tree must have ", queries, " words, got ", tree.size(0));
         TORCH_CHECK_VALUE(starts.defined() || seqs == 0 || queries / seqs <= 64, "a tree has at most 64 queried tokens per sequence, got ", queries / (seqs ? seqs : 1));
     }
-    const float scale = (float)float_arg(a[6]);
+    const float scale = (float)(a[6] == Py_None ? 1.0 / std::sqrt((double)p.dim) : float_arg(a[6]));
     const bool want_lse = a[7] == Py_True;
     Tensor out = optional_arg(a[8], "out"), lse;
     if (out.defined()) {

@@ -17,7 +17,6 @@ The cache is paged.  `pages` is int32 [n_pages, n_heads, page_size, words], made
 All of it is for inference: nothing here has a backward pass, and tensors that require gradients are refused outside torch.no_grad().  Calls only
 enqueue work on the current stream and may be captured into CUDA graphs.  (No counterpart in the reference.)
 """
-import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -78,8 +77,7 @@ def e8_cache_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor
 
     The call keeps a scratch buffer per device and stream, of 21 MB for heads of 64, 41 MB of 128, 10 MB of 256 (one per call that is captured into a graph, and
     on streams beyond the first 160 of a device)."""
-    return _lib.native().cache_attention(q, pages, table, lens, q_starts, tree, 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale),
-                                         bool(return_lse), out)
+    return _lib.native().cache_attention(q, pages, table, lens, q_starts, tree, None if scale is None else float(scale), bool(return_lse), out)
 
 
 class E8KVCache:

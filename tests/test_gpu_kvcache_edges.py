@@ -49,6 +49,18 @@ def test_rows_of_any_stride_where_a_dimension_is_one(dim, heads, n, dtype):
     assert torch.equal(kv.e8_cache_attention(apart, pages, t, lens), plainly)
 
 
+def test_queries_that_are_none_are_refused():
+    kv = api()
+    pages, table = filled(64, 2, 16, [20, 20], 5)
+    t, n = torch.tensor(table, dtype=torch.int32, device="cuda"), torch.tensor([20, 20], dtype=torch.int32, device="cuda")
+    for kind, q in ((TypeError, None), (TypeError, [1.0]), (ValueError, torch.zeros((), device="cuda")), (ValueError, torch.zeros(2, 4, 0, device="cuda")),
+                    (ValueError, torch.zeros(64, device="cuda"))):
+        with pytest.raises(kind, match="q must"):
+            kv.e8_cache_attention(q, pages, t, n)
+    q = rows(2, 4, 64, 3).cuda()
+    assert torch.equal(kv.e8_cache_attention(q, pages, t, n), kv.e8_cache_attention(q, pages, t, n, scale=0.125))
+
+
 # ------------------------------------------------------------------ streams
 def test_the_per_thread_default_stream_is_another_one_in_every_thread():
     """One handle, a stream for each thread: calls that run at the same time share nothing.  (The threads allocate nothing between their calls: PyTorch's
