@@ -260,3 +260,14 @@ def test_many_small_weights_beside_a_large_one(form, size):
     bound = (2.0 ** -22 + (dim + 32) * 2.0 ** -24) * 4 * s + 2.0 ** -20 + 2.0 ** -18 + 2.0 ** -22 * lse
     worst = float(((z.cpu().double() - lse).abs() / bound).max())
     assert worst <= 1.0, f"lse: {worst} of the bound"
+
+
+# ------------------------------------------------------------------ the benchmark
+def test_the_benchmark_sets_against_hbm_only_what_l2_cannot_hold():
+    from coset_b200 import benchmarks
+    l2 = torch.cuda.get_device_properties(0).L2_cache_size
+    records = list(benchmarks.iter_kvcache())
+    assert {r["bench"] for r in records} == {"kvcache_write", "kvcache_read", "kvcache_attention"}
+    for r in records:
+        assert r["ms"] > 0 and (r["inputs"] == "beyond L2") == (r["input_bytes"] >= 2 * l2) == ("frac_of_hbm" in r)
+        assert r.get("frac_of_hbm", 0.5) < 1.1
