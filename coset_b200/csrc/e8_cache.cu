@@ -286,7 +286,8 @@ bool known_dtype(int dtype) { return dtype == COSET_DTYPE_F32 || dtype == COSET_
 
 // The grid of a call, and whether its CTAs do two rounds: of bf16 tokens from four CTAs per SM on.  us with two rounds and with one, heads of 128: writing 8192
 // bf16 tokens of 8 heads 17.6 and 18.1, 32768 61.5 and 63.8, reading 32768 27.1 (96 % of the copy rate) and 28.2; writing 8192 float32 ones 18.8 and 19.7,
-// reading them 17.6 and 15.1.  Writes are bound by the issue of some 220 instructions per two blocks, reads by memory.
+// reading them 17.6 and 15.1.  Writes are bound by instructions, 430
+// for a thread's two blocks: issue slots 80 %, ALU pipe 71 %, most stalls on a pipe that is taken; reads (135) by memory.
 struct Shape {
     dim3 grid;
     bool twice;

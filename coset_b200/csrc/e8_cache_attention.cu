@@ -26,9 +26,9 @@
 // The running maximum is that of a weight times the size of its value (s + the exponent of the value's step), so that w = p step fits 16 bits: what is
 // lost is below 2^-31 of the row's largest (of a run of tokens that the tensor cores sum up, 2^-23 of the sum per token: they cut off what lies behind its 24 bits).  It follows only when it lags by 2^kSlack.  For float32 queries w is split into two 16-bit numbers.
 //
-// Measured, 8 heads of 128, 4 bf16 rows each: 32 sequences of 6144 tokens 62 us, of 12,288 112, of 24,576 210, so 4.4 TB/s of codes (two thirds of the copy rate)
+// Measured, 8 heads of 128, 4 bf16 rows each: 32 sequences of 6144 tokens 64 us, of 12,288 115, of 24,576 215, so 4.2 TB/s of codes (64 % of the copy rate)
 // beyond 13 us that a launch, the cut, the first loads and two joins cost.  A unit takes 700 instructions (values 250, keys 160, softmax 125, fetching 60): issue slots
-// 53 %, ALU pipe 44 %, tensor cores 29 %; twelve warps per SM instead of eight are not faster (67 and 70 us against 63 for lengths of 4000 to 8192).
+// 52 %, ALU pipe 44 %, tensor cores 29 %; twelve warps per SM instead of eight are not faster (67 and 70 us against 63 for lengths of 4000 to 8192).
 #include "e8_cache_attention.cuh"
 
 using namespace coset;
@@ -37,10 +37,13 @@ using namespace coset::cache;
 namespace {
 
 constexpr int kUnit = 32;         // tokens of a warp's step
-constexpr int kLeastUnits = 4;    // of a CTA
+// With kSegment, the least of the cut that a CTA has, counted in units and the segments' cost: one sequence of 1000 tokens and 8 heads, 8 times 32 units and 16 more, is
+// cut among 20 CTAs, of 3 to 20 units.
+constexpr int kLeastUnits = 4;
 constexpr int kQueryBytes = 3;         // of a query in fixed point
 constexpr int kExact = 0x4B400000;  // the bits of kExactly = 1.5 2^23; a whole number of up to 22 bits added to them is added to it
-// What a segment costs a CTA beyond its units, in units: its queries, its first loads' latency, its joining.  The cut counts it.  (32 sequences of 4000 to 8192
+// What a segment costs a CTA beyond its units, in units: its queries, its first loads' latency, its joining.  The cut counts it once per segment, behind its last
+// unit, though each of several CTAs that share one pays for it.  (32 sequences of 4000 to 8192
 // tokens: 63 us, with 24 64, with 32 66; one sequence of 131,071 55, 53, 53.)
 constexpr int kSegment = 16;
 
@@ -694,13 +697,14 @@ int launch_as(const Attend& a, cudaStream_t st) {
 // Up to so many rows of a cache head, on average over the sequences, stay here; bf16 queries with more go to the kernel for many.  8 cache heads, us here and
 // there: of 128 values, 8 sequences of 500 to 3000 tokens with 16, 24, 32 rows 26 and 27, 32 and 27, 36 and 28; 4 of 8000 to 16384 45 and 53, 61 and 53, 64 and
 // 55; 32 of 3000 to 6000 84 and 138, 146 and 139, 153 and 140; of 64 values, 8 of 500 to 3000 with 24, 32, 64 rows 22 and 24, 24 and 24, 35 and 25; 32 of 3000 to
-// 6000 with 24, 32 rows 97 and 114, 100 and 115.
+// 6000 with 24, 32 rows 97 and 114, 100 and 115.  A batch goes to one kernel as a whole: 63 single tokens and a chain of 16, 64, 512 over 3000 tokens each take 77, 100 and
+// 240 us in one call, 66 and 26, 55, 77 in a call each.
 constexpr int few_rows_at_most(int head_dim) { return head_dim == 64 ? 32 : 16; }
 
 template <int DIM, bool BF16>
 int launch(const Attend& a, cudaStream_t st) {
     const int64_t rows = ((int64_t)a.n_queries + a.n_seqs - 1) / a.n_seqs * a.group;  // of a cache head, on average
-    // 256 values of 16 queries do not fit a thread's registers: 8 sequences of 500 to 3000 tokens with 16 rows 49 us in one tile, 36 in two of 8; 128 rows 166, 147
+    // 16 queries of 128 values take all registers of a thread and 60 to 72 bytes more; 256 values of 16 do not fit at all: 8 sequences of 500 to 3000 tokens with 16 rows 49 us in one tile, 36 in two of 8; 128 rows 166, 147
     if constexpr (DIM == 256) return launch_as<DIM, BF16, 1, 6, 1>(a, st);
     // Fewer parts to join where few heads' tokens are shared by all CTAs, more overlap of one CTA's joining with the other's units elsewhere.  us with one CTA of 8
     // warps and with two of 4: 8 heads of 131,071 tokens 49 and 55, of 32,000 19.7 and 20.5, 2 heads of 32,000 16.5 and 19.1; 64 of 4000 to 8000 24.2 and 22.8,

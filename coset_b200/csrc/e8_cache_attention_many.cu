@@ -12,9 +12,9 @@
 // codes are decoded once for both (PAIR).  The running maximum follows only when it lags by 2^kSlack, so O is seldom scaled.  Work is cut among the CTAs
 // as for few rows.
 //
-// Measured: 4 sequences of 8000 to 16384 tokens, 64 queries of 8 heads per cache head, 8 cache heads of 128: 196 us, 0.56 PFLOP/s of S and O.  A group's turn of
-// 128 queries by 128 tokens takes some 6300 cycles: 1450 for the maxima, 2700 for the weights, 1900 until the next S.  No unit is full (issue slots 43 %,
-// shared memory's pipe 57 %, tensor cores 28 %): what bounds it is the softmax's chain of dependent instructions in two warps per scheduler.  Without any one
+// Measured: 4 sequences of 8000 to 16384 tokens, 64 queries of 8 heads per cache head, 8 cache heads of 128: 195 us, 0.59 PFLOP/s of S and O.  A group's turn of
+// 128 queries by 128 tokens takes some 6300 cycles: 1450 for the maxima, 2700 for the weights, 1900 until the next S.  No unit is full (issue slots 42 %,
+// shared memory's pipe 55 %, tensor cores 28 %): what bounds it is the softmax's chain of dependent instructions in two warps per scheduler.  Without any one
 // of decoding, maxima, weights, loads of steps it would be 3 to 15 % faster.  Tried: one group with halves of rows 232 us; eight decoding warps and registers
 // moved to the softmax 197; loops over tokens unrolled by two or with tensor memory's loads ahead 196 and 235, by 16 instead of 32 tokens 205.
 //
@@ -33,7 +33,7 @@ namespace {
 
 constexpr int kTileRows = 128, kTile = 128;  // queries and tokens of a tile
 constexpr int kLeastPage = 16;           // tokens of a page
-// A segment's cost beyond its tiles, in tiles, and the least that a CTA does.  4 sequences of 8000 to 16384 tokens with 512 rows 194 us (2 tiles: 200, 8: 197), 32 of 3000 to
+// A segment's cost beyond its tiles, in tiles, and, with it, the least of the cut that a CTA has.  4 sequences of 8000 to 16384 tokens with 512 rows 194 us (2 tiles: 200, 8: 197), 32 of 3000 to
 // 6000 with 32 rows 140 (139, 145); 2 of 300 to 600 with 28 rows 17.9 us (at least 1 tile: 18.4, 4: 23.4).
 constexpr int kSegment = 4, kLeastTiles = 2;
 constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4, kProductWarp = kSoftmaxWarps + kDecodeWarps, kThreads = 32 * (kProductWarp + 1);

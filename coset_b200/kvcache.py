@@ -72,8 +72,9 @@ def e8_cache_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor
 
     A query that sees nothing gives zeros (and -inf).  Queries count with 24 bits from the largest of their row on, sums and the softmax's statistics are
     float32, and weights are rounded to 11 bits for bf16 queries, to 22 for float32 ones.  Where a tree's or a chain's queries of a cache head are
-    more than 16 (32 of 64 values) on average, bf16 products run on tcgen05 and sum in another order: results agree to the rounding, not to the bit.  Equal
-    calls give equal bits.  Of values above 7e31 small weights are lost: those below 2^-29 of the largest one there, below 2^-20 at 3e34, 2^-7 at 3e38.
+    more than 16 (32 of 64 values) on average over the sequences, bf16 products run on tcgen05 and sum in another order: results agree to the rounding, not
+    to the bit.  (A long chain beside many single tokens is faster in a call of its own.)  Equal calls give equal bits.  Of values above 7e31 small
+    weights are lost: those below 2^-29 of the largest one there, below 2^-20 at 3e34, 2^-7 at 3e38.
 
     The call keeps a scratch buffer per device and stream, of 21 MB for heads of 64, 41 MB of 128, 10 MB of 256 (one per call that is captured into a graph, and
     on streams beyond the first 160 of a device)."""
