@@ -24,7 +24,8 @@
 // order of the CTAs.
 //
 // The running maximum is that of a weight times the size of its value (s + the exponent of the value's step), so that w = p step fits 16 bits: what is
-// lost is below 2^-31 of the row's largest (of a run of tokens that the tensor cores sum up, 2^-23 of the sum per token: they cut off what lies behind its 24 bits).  It follows only when it lags by 2^kSlack.  For float32 queries w is split into two 16-bit numbers.
+// lost is below 2^-31 of the row's largest (and, in a run of tokens that the tensor cores sum up, 2^-23 of the sum per token: they cut off what lies behind its 24
+// bits).  It follows only when it lags by 2^kSlack.  For float32 queries w is split into two 16-bit numbers.
 //
 // Measured, 8 heads of 128, 4 bf16 rows each: 32 sequences of 6144 tokens 64 us, of 12,288 115, of 24,576 215, so 4.2 TB/s of codes (64 % of the copy rate)
 // beyond 13 us that a launch, the cut, the first loads and two joins cost.  A unit takes 700 instructions (values 250, keys 160, softmax 125, fetching 60): issue slots
@@ -43,8 +44,8 @@ constexpr int kLeastUnits = 4;
 constexpr int kQueryBytes = 3;         // of a query in fixed point
 constexpr int kExact = 0x4B400000;  // the bits of kExactly = 1.5 2^23; a whole number of up to 22 bits added to them is added to it
 // What a segment costs a CTA beyond its units, in units: its queries, its first loads' latency, its joining.  The cut counts it once per segment, behind its last
-// unit, though each of several CTAs that share one pays for it.  (32 sequences of 4000 to 8192
-// tokens: 63 us, with 24 64, with 32 66; one sequence of 131,071 55, 53, 53.)
+// unit, though each of several CTAs that share one pays for it.  (32 sequences of 4000 to 8192 tokens: 63 us, with 24 64, with 32 66; one sequence of 131,071
+// 55, 53, 53.)
 constexpr int kSegment = 16;
 
 // The row of a group of 8 that stands in row r of an operand: 0 1 2 3 5 4 7 6.  With the swizzle below no read of codes has a bank conflict.
@@ -704,7 +705,8 @@ constexpr int few_rows_at_most(int head_dim) { return head_dim == 64 ? 32 : 16; 
 template <int DIM, bool BF16>
 int launch(const Attend& a, cudaStream_t st) {
     const int64_t rows = ((int64_t)a.n_queries + a.n_seqs - 1) / a.n_seqs * a.group;  // of a cache head, on average
-    // 16 queries of 128 values take all registers of a thread and 60 to 72 bytes more; 256 values of 16 do not fit at all: 8 sequences of 500 to 3000 tokens with 16 rows 49 us in one tile, 36 in two of 8; 128 rows 166, 147
+    // 16 queries of 128 values take all registers of a thread and 60 to 72 bytes more; 256 values of 16 do not fit at all: 8 sequences of 500 to 3000 tokens with
+    // 16 rows 49 us in one tile, 36 in two of 8; 128 rows 166, 147
     if constexpr (DIM == 256) return launch_as<DIM, BF16, 1, 6, 1>(a, st);
     // Fewer parts to join where few heads' tokens are shared by all CTAs, more overlap of one CTA's joining with the other's units elsewhere.  us with one CTA of 8
     // warps and with two of 4: 8 heads of 131,071 tokens 49 and 55, of 32,000 19.7 and 20.5, 2 heads of 32,000 16.5 and 19.1; 64 of 4000 to 8000 24.2 and 22.8,

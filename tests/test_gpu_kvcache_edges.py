@@ -9,6 +9,7 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import kvcache_util as plain
 from test_gpu_kvcache import DTYPES, api, as_words, check, expected_pages, filled, rows
 
 pytestmark = pytest.mark.gpu
@@ -199,6 +200,27 @@ def test_values_of_every_size(form, size):
     pages, table = with_values(dim, L, v)
     q = rows(2, group, dim, 32, DTYPES[dtype]).cuda()
     check(q, pages, dim, table, [L], [0, 2], None)
+
+
+@pytest.mark.parametrize("size", [1e33, 1e35, 1e37, 1e38])
+@pytest.mark.parametrize("form", FORMS, ids=FORM)
+def test_values_near_the_end_of_the_type(form, size):
+    """Above 7e31 small weights are lost and sums have fewer bits: of 300 weights as large as each other, as zero keys make them, at most 2^-17 each by then."""
+    dtype, dim, group = form
+    L = 300
+    v = rows(L, 1, dim, 31)[:, 0].clamp(-3, 3) * size
+    v[:, 0] = 3.0 * size
+    pages, table = with_values(dim, L, v)
+    kc, kh, vc, vh = plain.planes(as_words(pages), dim)
+    q = torch.zeros(2, group, dim, dtype=DTYPES[dtype], device="cuda")
+    y, z = api().e8_cache_attention(q, pages, torch.tensor(table, dtype=torch.int32, device="cuda"), torch.tensor([L], dtype=torch.int32, device="cuda"), return_lse=True)
+    at = [(table[0][i // 16], i % 16) for i in range(L)]
+    vd = torch.stack([plain.values(vc[p, 0, r], vh[p, 0, r]) for p, r in at])
+    for i, n in ((0, L - 1), (1, L)):  # a chain of two
+        want, spread = vd[:n].mean(0), vd[:n].abs().mean(0)
+        bound = torch.finfo(DTYPES[dtype]).eps / 2 * want.abs() + (2.0 ** -18 + 2.0 ** -17) * spread
+        assert ((y[i].cpu().double() - want).abs() <= bound).all()
+        assert ((z[i].cpu().double() - math.log(n)).abs() <= 2.0 ** -17 + 2.0 ** -20).all()
 
 
 @pytest.mark.parametrize("form", FORMS, ids=FORM)
