@@ -124,6 +124,39 @@ def test_streams_that_come_and_go():
     assert most <= 2 ** 20  # nothing is kept for the last 200
 
 
+@pytest.mark.parametrize("dim, dtype, tokens", [(128, "bf16", 1), (64, "f32", 3), (128, "bf16", 40), (256, "bf16", 2)])
+def test_the_first_call_of_a_process_may_be_captured(dim, dtype, tokens):
+    import subprocess
+    child = os.path.join(os.path.dirname(os.path.abspath(__file__)), "kvcache_capture_child.py")
+    done = subprocess.run([sys.executable, child, str(dim), dtype, str(tokens)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip().endswith("ok"), done.stdout + done.stderr
+
+
+@pytest.mark.parametrize("tokens", [1, 9, 40])
+def test_a_capture_that_forks_into_two_streams(tokens):
+    """Two calls side by side in one graph, and one behind both."""
+    kv = api()
+    dim = 128
+    pages, table = filled(dim, 2, 16, [900, 300], 5)
+    t, lens = torch.tensor(table, dtype=torch.int32, device="cuda"), torch.tensor([100, 60], dtype=torch.int32, device="cuda")
+    qs = [rows(2 * tokens, 8, dim, s, torch.bfloat16).cuda() for s in range(3)]
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        got = [kv.e8_cache_attention(qs[0], pages, t, lens)]
+        with torch.cuda.stream(side):
+            got.append(kv.e8_cache_attention(qs[1], pages, t, lens))
+        main.wait_stream(side)
+        got.append(kv.e8_cache_attention(qs[2], pages, t, lens))
+    for now in ([900, 300], [64, 64], [577, 1]):
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        for _ in range(20):
+            graph.replay()
+        for q, y in zip(qs, got):
+            assert torch.equal(y, kv.e8_cache_attention(q, pages, t, lens))
+
+
 # ------------------------------------------------------------------ long sums
 LONG = [("f32", 128, 1, 1), ("f32", 64, 2, 5), ("f32", 256, 1, 1), ("bf16", 128, 4, 1), ("bf16", 128, 4, 3), ("bf16", 256, 2, 1), ("bf16", 64, 8, 5), ("bf16", 64, 8, 32),
         ("bf16", 128, 8, 16), ("bf16", 128, 8, 32)]
